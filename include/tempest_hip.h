@@ -543,7 +543,7 @@ int th_build_tanh_layer_grad(int32_t d, int32_t h, int32_t c,
 
 /* ---- op class (b): bf16 products on the matrix cores --------------------- */
 
-enum { TH_F32 = 0, TH_BF16 = 1, TH_I32 = 2, TH_I64 = 3, TH_F16 = 4 };
+enum { TH_F32 = 0, TH_BF16 = 1, TH_I32 = 2, TH_I64 = 3, TH_F16 = 4, TH_E4M3 = 5 };
 
 /* What the product's group fuses after it.  Every epilogue works on the fp32
  * accumulator and rounds once to bf16 where it stores, except where noted.
@@ -733,6 +733,151 @@ int th_build_attention_fwd(const th_attention_desc* desc, th_launch** host_out);
  * 10 lengths.  Replaces the
  * cuTile transposed folds of the backward (ext/cuTileExt/transpose.jl:1-213). */
 int th_build_attention_bwd(const th_attention_desc* desc, th_launch** host_out);
+
+/* ---- rotary positions ------------------------------------------------------ */
+
+/* q and k turned by their positions, on any number of axes (a text's running
+ * position; an image's rows and columns; a film's time, height and width):
+ * pair p of the first rotary_dim features of a head turns by
+ *   theta_p = positions[axis(p), s, b] * freqs[p],
+ * (u, v) to (u cos theta - v sin theta, u sin theta + v cos theta), the features
+ * behind rotary_dim passing as they are.  Pair p is features p and p +
+ * rotary_dim / 2, or, with TH_ROTARY_PAIRS, 2p and 2p + 1; the first sections[0]
+ * pairs turn with axis 0, the next sections[1] with axis 1, and so on.  theta is
+ * formed and reduced in 64 bits, so that a position of any size keeps its turn;
+ * the products are fp32, rounded once to the arrays' type.  With
+ * TH_ROTARY_INVERSE everything turns back (by -theta), which is the gradient:
+ * dq of q from that of the turned q.
+ * Arrays are (d, heads, positions, batch), fp32, bf16 or fp16, at strides along
+ * heads, positions and batch (elements, features adjacent); any alignment.  q_out may be
+ * q (its strides q's), k_out k; otherwise outputs overlap no input.  kv_heads 0: no k.
+ * positions is int32, element (axis, s, b) at position_strides (0 where an axis
+ * of the array is broadcast), freqs fp32, rotary_dim / 2 of them.
+ * Values: 0 q, 1 k, 2 q_out, 3 k_out, 4 positions, 5 freqs.  No counterpart in
+ * the reference, whose programs would spell it as a pointwise group. */
+#define TH_ROTARY_AXES 4
+#define TH_ROTARY_PAIRS 1
+#define TH_ROTARY_INVERSE 2
+typedef struct th_rotary_desc {
+  int32_t dtype; /* TH_F32, TH_BF16 or TH_F16 */
+  int32_t batch, seq, heads, kv_heads, head_dim;
+  int32_t rotary_dim; /* even, at most head_dim */
+  int32_t axes;       /* 1..TH_ROTARY_AXES */
+  int32_t sections[TH_ROTARY_AXES]; /* pairs of each axis, rotary_dim / 2 in all */
+  int32_t flags;      /* TH_ROTARY_* */
+  int32_t reserved;
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_strides[3]; /* along heads, positions, batch */
+  int64_t k_strides[3];
+  int64_t q_out_strides[3];
+  int64_t k_out_strides[3];
+  const int32_t* positions;
+  const float* freqs;
+  int64_t position_strides[3]; /* along axes, positions, batch */
+} th_rotary_desc;
+
+int th_build_rotary(const th_rotary_desc* desc, th_launch** host_out);
+
+/* ---- a key-value cache in pages --------------------------------------------- */
+
+/* K and V arrays (features, heads, positions in a page, pages), bf16, fp16 or
+ * e4m3, at strides along heads, positions and pages (elements, features
+ * adjacent; one stride set for both, heads and positions in either order).
+ * head_dim is a multiple of 8 up to 256, the arrays 16-byte aligned, strides
+ * multiples of 8.
+ * TH_E4M3: a byte a feature, and for each 32 features of a row one byte e, the scale
+ * 2^(e - 127): what is held is the code's value times the scale.  The scale of
+ * the feature at element x of k is k_scales[x / 32], so head_dim and the strides are
+ * multiples of 32.
+ * A sequence's position p is in page table[p / page, b] at place p % page:
+ * table is int32 (table_pages, batch), entry i of sequence b at i +
+ * table_pages * b.  An entry outside 0..pages-1 names no page: nothing is
+ * written there, what is read there is zero, and no query sees a key there.
+ * lengths, int32 (batch), is how many positions each sequence holds, new ones
+ * included (taken into 0..table_pages * page); counts, int32 (batch) or NULL, how
+ * many of the seq new ones are real (into 0..seq; NULL: all seq): the j-th new
+ * position of sequence b is lengths[b] - counts[b] + j.  The device holds table,
+ * lengths and counts and reads them when the launch runs.
+ * No counterpart in the reference, whose decode reads dense arrays
+ * (test/cuda/attention.jl:254-271). */
+typedef struct th_cache {
+  int32_t dtype; /* TH_BF16, TH_F16 or TH_E4M3 */
+  int32_t heads, head_dim;
+  int32_t page;  /* positions a page: any number */
+  int32_t pages; /* pages in the arrays; pages * page under 2^31 */
+  int32_t reserved;
+  void* k;
+  void* v;
+  uint8_t* k_scales; /* TH_E4M3 only */
+  uint8_t* v_scales;
+  int64_t strides[3]; /* along heads, positions in a page, pages */
+} th_cache;
+
+/* Dense rows to or from the cache: k and v (d, heads, positions, batch) of
+ * `dtype` at strides along heads, positions, batch; any alignment. */
+typedef struct th_cache_desc {
+  th_cache cache;
+  int32_t dtype; /* of k and v: the cache's, or TH_BF16 or TH_F16 beside TH_E4M3 */
+  int32_t batch, seq, table_pages;
+  void* k;
+  void* v;
+  int64_t strides[3];
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* counts; /* writing only */
+} th_cache_desc;
+
+/* Write the new positions' rows k and v (positions 0..counts[b]-1 of sequence
+ * b) into the cache; rows at a position below 0, and what no new position names, stay.
+ * TH_E4M3: each 32 features x become codes of x / 2^s, s the least integer for which
+ * the largest finite |x| is at most 448 * 2^s, rounded once to nearest, ties
+ * to even; s is at least -117 (every value held is a normal number) and at
+ * most 119 (7 for fp16 rows; 448 * 2^s stays finite in the rows' type), beyond
+ * which codes saturate at 448; NaN and infinities become NaN.  Two positions in one page's place leave
+ * either's bytes there.
+ * Values: 0 k, 1 v, 2 the cache's k, 3 its v, 4 k_scales, 5 v_scales, 6 table,
+ * 7 lengths, 8 counts. */
+int th_build_cache_write(const th_cache_desc* desc, th_launch** host_out);
+
+/* Read positions 0..min(lengths[b], seq)-1 of each sequence back into k and v,
+ * as th_build_attention_fwd takes them; rows behind them stay.  TH_E4M3: the values held,
+ * rounded once to k's type.  Values: as th_build_cache_write's, without counts. */
+int th_build_cache_read(const th_cache_desc* desc, th_launch** host_out);
+
+/* o = softmax(scale * k'q, masked) * v over a cache in pages, for seq new
+ * positions a sequence (one when decoding, a few when proposals are checked): query j of
+ * sequence b, at position p = lengths[b] - counts[b] + j, sees keys 0..lengths[b]-1,
+ * causal only those up to p, and with a window (causal only) those after p - window.
+ * A query that sees no key gets o = 0 and lse = -inf; rows j >=
+ * counts[b] of o and lse stay.  What a key or value holds that no query sees may be
+ * anything, NaN included.
+ * q and o are (d, heads, positions, batch) at q_strides, bf16 or fp16, the cache's
+ * type or beside TH_E4M3; any alignment.  lse (if non-NULL) as th_build_attention_fwd
+ * writes it; heads a multiple of the cache's heads; scale <= 0 means
+ * 1/sqrt(head_dim).  The weights are fp32's, as are all sums.  The keys are read once for
+ * every 16 rows (seq * heads / cache heads).  Workspace: the split's partial results.
+ * Values: 0 q, 1 o, 2 lse, 3 the cache's k, 4 its v, 5 k_scales, 6 v_scales,
+ * 7 table, 8 lengths, 9 counts. */
+typedef struct th_paged_desc {
+  th_cache cache;
+  int32_t dtype; /* of q and o */
+  int32_t batch, heads, seq, table_pages;
+  int32_t causal;
+  int32_t window; /* 0: none */
+  float scale;
+  const void* q;
+  void* o;
+  float* lse;
+  int64_t q_strides[3]; /* along heads, positions, batch */
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* counts;
+} th_paged_desc;
+
+int th_build_attention_paged(const th_paged_desc* desc, th_launch** host_out);
 
 /* ---- config 5: chunked gated DeltaNet (scan + recurrence) ---------------- */
 

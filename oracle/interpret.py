@@ -352,3 +352,97 @@ def deltanet_grad(q, k, v, a, beta, do, C=64):
     dca[..., -1] += kd.sum(-1) + dg * c["g"]
     da = np.flip(np.cumsum(np.flip(dca, -1), -1), -1)
     return _unchunks(dQ), _unchunks(dK), _unchunks(dV), _unchunks(da), _unchunks(dBt)
+
+
+# ---- rotary positions and a key-value cache in pages -------------------------
+
+def rotary(x, positions, freqs, sections, pairs=False, inverse=False):
+    """x (batch, positions, heads, d) turned: pair p of the first 2 len(freqs)
+    features by positions[..., axis(p)] * freqs[p] (back with inverse); pair p is
+    features p and p + len(freqs), or with `pairs` 2p and 2p + 1.  positions
+    (batch, positions, axes); sections: pairs of each axis, in order."""
+    x, freqs = _f64(x).copy(), _f64(freqs)
+    n = len(freqs)
+    axis = np.repeat(np.arange(len(sections)), sections)
+    theta = (_f64(positions)[..., axis] * freqs)[:, :, None, :] * (-1.0 if inverse else 1.0)
+    lo = slice(0, 2 * n, 2) if pairs else slice(0, n)
+    hi = slice(1, 2 * n, 2) if pairs else slice(n, 2 * n)
+    u, v = x[..., lo].copy(), x[..., hi].copy()
+    x[..., lo] = u * np.cos(theta) - v * np.sin(theta)
+    x[..., hi] = u * np.sin(theta) + v * np.cos(theta)
+    return x
+
+
+def e4m3_values():
+    """What the 256 codes of e4m3 stand for: 1 sign bit, 4 of exponent (bias 7),
+    3 of mantissa; exponent 0 holds steps of 2^-9, and 0x7f, 0xff are NaN."""
+    out = np.empty(256)
+    for code in range(256):
+        e, m = code >> 3 & 15, code & 7
+        v = m * 2.0 ** -9 if e == 0 else (8 + m) * 2.0 ** (e - 10)
+        out[code] = np.nan if code & 127 == 127 else -v if code & 128 else v
+    return out
+
+
+def e4m3_rows(x, fp16=False):
+    """(codes, scale bytes) of x (..., d): for each 32 features the scale 2^s for
+    the least s with the largest finite |x| <= 448 * 2^s, s in -117..119 (..7
+    for fp16 rows), and the code nearest x / 2^s, even codes between two; beyond
+    448 the code of 448, NaN where x is not finite.  By search over the codes."""
+    x = _f64(x).reshape(*np.shape(x)[:-1], -1, 32)
+    finite = np.where(np.isfinite(x), np.abs(x), 0.0)
+    top = finite.max(-1)
+    most = 7 if fp16 else 119
+    s = np.full(top.shape, -117)
+    for k in range(-116, most + 1):
+        s = np.where(top > 448.0 * 2.0 ** (k - 1), k, s)
+    grid = e4m3_values()[:127]
+    y = np.minimum(finite / 2.0 ** s[..., None], 448.0)
+    hi = np.searchsorted(grid, y)  # grid[hi - 1] < y <= grid[hi]
+    lo = np.maximum(hi - 1, 0)
+    below, above = y - grid[lo], grid[hi] - y
+    code = np.where((below < above) | ((below == above) & (lo % 2 == 0)), lo, hi)
+    code = np.where(np.isfinite(x), code | np.where(np.signbit(x), 128, 0), 127)
+    return code.reshape(*x.shape[:-2], -1).astype(np.uint8), (s + 127).astype(np.uint8)
+
+
+def e4m3_held(codes, scales):
+    """What codes (..., d) and their scale bytes (..., d / 32) stand for."""
+    v = e4m3_values()[codes].reshape(*codes.shape[:-1], -1, 32)
+    return (v * 2.0 ** (scales.astype(np.float64) - 127)[..., None]).reshape(codes.shape)
+
+
+def paged_attention(q, k, v, lengths, counts=None, causal=True, window=0, scale=None, present=None):
+    """(o, lse, rows there): q (batch, seq, heads, d) at the end of sequences whose
+    keys k and v (batch, positions, kv_heads, d) are in order.  Query j of batch b, at
+    position p = lengths[b] - counts[b] + j, sees keys i < lengths[b], causal
+    those i <= p, with a window those i > p - window, and only those with
+    present[b, i]; a row that sees none is 0, its lse -inf."""
+    q, k, v = _f64(q), _f64(k), _f64(v)
+    B, S, H, D = q.shape
+    group = H // k.shape[2]
+    scale = scale or 1.0 / np.sqrt(D)
+    o, lse, there = np.zeros_like(q), np.full((B, S, H), -np.inf), np.zeros((B, S), bool)
+    for b in range(B):
+        n = S if counts is None else min(max(int(counts[b]), 0), S)
+        there[b, :n] = True
+        key = np.arange(min(max(int(lengths[b]), 0), k.shape[1]))
+        for j in range(n):
+            p = len(key) - n + j
+            see = np.ones(len(key), bool)
+            if causal:
+                see &= key <= p
+            if window:
+                see &= key > p - window
+            if present is not None:
+                see &= present[b, :len(key)]
+            at = key[see]
+            if len(at) == 0:
+                continue
+            for h in range(H):
+                s = k[b, at, h // group] @ q[b, j, h] * scale
+                top = s.max()
+                w = np.exp(s - top)
+                lse[b, j, h] = top + np.log(w.sum())
+                o[b, j, h] = (w / w.sum()) @ v[b, at, h // group]
+    return o, lse, there

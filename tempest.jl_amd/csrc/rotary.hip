@@ -1,0 +1,239 @@
+// Rotary positions on several axes: q and k turned pair by pair, fp32, bf16
+// or fp16.  Memory-bound: every element is read once and written once.
+//
+// A workgroup takes a few tokens with all their heads: its threads first form
+// the tokens' cosines and sines (rotary_dim / 2 a token, shared by all heads)
+// in LDS, then each turns V pairs at a time, 16 bytes of either half.
+//
+// The angle is position * frequency, in turns t = position * (freq / 2 pi) in
+// fp64 (two roundings: off by at most 2^-52 t, so by 2^-21 of a turn at 2^31 turns);
+// t - rint(4 t) / 4, in [-1/8, 1/8], is exact and goes on in fp32, where
+// Taylor's polynomials of sin and cos on [-pi/4, pi/4] leave out under 2^-28.
+#include <hip/hip_runtime.h>
+
+#include "th_core.h"
+
+namespace {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+struct RotaryArray {
+  const void* x;
+  void* y;
+  int64_t xh, xs, xb, yh, ys, yb;
+  int32_t heads;
+};
+
+struct RotaryArgs {
+  RotaryArray a[2];  // q, k
+  const int32_t* positions;
+  const float* freqs;
+  int64_t pa, ps, pb;  // the positions' strides along axes, positions, batch
+  int64_t tokens;      // seq * batch
+  int32_t seq, half;   // half: pairs a head
+  int32_t ends[TH_ROTARY_AXES];  // pair p turns with the first axis whose end passes it
+  int32_t turning, passing;      // items of a head: turned, copied
+  int32_t per_block;             // tokens a workgroup
+  float sign;
+};
+
+// sin and cos of 2 pi t.
+__device__ __forceinline__ float2 turned(double t) {
+  const double n = rint(4.0 * t);
+  const float x = 6.283185307179586f * (float)(t - 0.25 * n);
+  const float y = x * x;
+  float s = fmaf(y, 2.7557319e-6f, -1.9841270e-4f);
+  s = fmaf(y, s, 8.3333333e-3f);
+  s = fmaf(y, s, -1.6666667e-1f);
+  s = fmaf(x * y, s, x);
+  float c = fmaf(y, -2.7557319e-7f, 2.4801587e-5f);
+  c = fmaf(y, c, -1.3888889e-3f);
+  c = fmaf(y, c, 4.1666667e-2f);
+  c = fmaf(y, c, -0.5f);
+  c = fmaf(y, c, 1.0f);
+  const int quarter = (int)(n - 4.0 * rint(0.25 * n)) & 3;
+  const float u = quarter & 1 ? c : s, v = quarter & 1 ? s : c;
+  return {quarter & 2 ? -u : u, (quarter + 1) & 2 ? -v : v};
+}
+
+template <int T>  // TH_F32, TH_BF16, TH_F16
+struct Element {
+  typedef uint16_t type;
+};
+template <>
+struct Element<TH_F32> {
+  typedef float type;
+};
+
+template <int T>
+__device__ __forceinline__ float wide(typename Element<T>::type x) {
+  if constexpr (T == TH_F32) return x;
+  if constexpr (T == TH_BF16) return __uint_as_float((uint32_t)x << 16);
+  if constexpr (T == TH_F16) return (float)__builtin_bit_cast(_Float16, x);
+}
+template <int T>
+__device__ __forceinline__ typename Element<T>::type narrow(float x) {
+  if constexpr (T == TH_F32) return x;
+  if constexpr (T == TH_BF16) return __builtin_bit_cast(uint16_t, (__bf16)x);
+  if constexpr (T == TH_F16) return __builtin_bit_cast(uint16_t, (_Float16)x);
+}
+
+// V elements at the elements' own alignment.
+template <class E, int V>
+struct __attribute__((packed, aligned(sizeof(E)))) Vec {
+  E x[V];
+};
+
+template <int T, int V, bool PAIRS>
+__global__ __launch_bounds__(256) void rotary(RotaryArgs p) {
+  typedef typename Element<T>::type E;
+  typedef Vec<E, V> W;
+  extern __shared__ float2 turns[];  // [token][pair]: sin, cos
+  const int64_t first = (int64_t)blockIdx.x * p.per_block;
+  const int tokens = (int)min((int64_t)p.per_block, p.tokens - first);
+  for (int i = threadIdx.x; i < tokens * p.half; i += 256) {
+    const int t = i / p.half, pair = i - t * p.half;
+    const int64_t token = first + t, b = token / p.seq, s = token - b * p.seq;
+    int axis = 0;
+#pragma unroll
+    for (int a = 0; a < TH_ROTARY_AXES - 1; ++a) axis += pair >= p.ends[a];
+    const int position = p.positions[axis * p.pa + s * p.ps + b * p.pb];
+    turns[i] = turned((double)position * ((double)p.freqs[pair] * 0.15915494309189535));
+  }
+  __syncthreads();
+  const int per_head = p.turning + p.passing;
+  const int per_token = (p.a[0].heads + p.a[1].heads) * per_head;
+  for (int i = threadIdx.x; i < tokens * per_token; i += 256) {
+    const int t = i / per_token, at = i - t * per_token;
+    int head = at / per_head;
+    const int item = at - head * per_head;
+    const bool second = head >= p.a[0].heads;
+    const RotaryArray& a = p.a[second];
+    if (second) head -= p.a[0].heads;
+    const int64_t token = first + t, b = token / p.seq, s = token - b * p.seq;
+    const E* x = static_cast<const E*>(a.x) + head * a.xh + s * a.xs + b * a.xb;
+    E* y = static_cast<E*>(a.y) + head * a.yh + s * a.ys + b * a.yb;
+    if (item >= p.turning) {
+      const int f = 2 * p.half + V * (item - p.turning);
+      *reinterpret_cast<W*>(y + f) = *reinterpret_cast<const W*>(x + f);
+      continue;
+    }
+    const int f0 = PAIRS ? 2 * V * item : V * item, f1 = PAIRS ? f0 + V : f0 + p.half;
+    W u = *reinterpret_cast<const W*>(x + f0), v = *reinterpret_cast<const W*>(x + f1);
+    const float2* turn = turns + t * p.half + V * item;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      // Pair j: in halves element j of either, adjacent ones elements 2j and 2j + 1 of both together.
+      E& lo = PAIRS ? (2 * j < V ? u.x[2 * j] : v.x[2 * j - V]) : u.x[j];
+      E& hi = PAIRS ? (2 * j + 1 < V ? u.x[2 * j + 1] : v.x[2 * j + 1 - V]) : v.x[j];
+      const float sin = p.sign * turn[j].x, cos = turn[j].y;
+      const float g = wide<T>(lo), h = wide<T>(hi);
+      lo = narrow<T>(g * cos - h * sin);
+      hi = narrow<T>(g * sin + h * cos);
+    }
+    *reinterpret_cast<W*>(y + f0) = u;
+    *reinterpret_cast<W*>(y + f1) = v;
+  }
+}
+
+template <int T, int V>
+const void* kernel_of(bool pairs) {
+  return pairs ? (const void*)rotary<T, V, true> : (const void*)rotary<T, V, false>;
+}
+template <int T>
+const void* kernel_of(int v, bool pairs) {
+  if constexpr (T != TH_F32)
+    if (v == 8) return kernel_of<T, 8>(pairs);
+  return v == 4 ? kernel_of<T, 4>(pairs) : v == 2 ? kernel_of<T, 2>(pairs) : kernel_of<T, 1>(pairs);
+}
+
+int check_array(const void* x, void* y, const int64_t* xs, const int64_t* ys, const th_rotary_desc* d, int heads,
+                int size) {
+  TH_REQUIRE(x && y, "rotary: null q, k, q_out or k_out");
+  TH_REQUIRE(reinterpret_cast<uintptr_t>(x) % size == 0 && reinterpret_cast<uintptr_t>(y) % size == 0,
+             "rotary: arrays must be aligned to their elements");
+  const int64_t extents[3] = {heads, d->seq, d->batch};
+  for (int i = 0; i < 3; ++i) TH_REQUIRE(xs[i] >= 0 && ys[i] >= 0, "rotary: strides must not be negative");
+  TH_REQUIRE(th::rows_apart(d->head_dim, ys, extents, 3), "rotary: the output's rows overlap");
+  for (int i = 0; i < 3; ++i)
+    TH_REQUIRE(x != y || extents[i] == 1 || xs[i] == ys[i], "rotary: an array turned in place keeps its strides");
+  return TH_OK;
+}
+
+int build(const th_rotary_desc* d, th_launch** out) {
+  TH_REQUIRE(d != nullptr, "rotary: null descriptor");
+  if (d->dtype != TH_F32 && d->dtype != TH_BF16 && d->dtype != TH_F16)
+    return th::fail(TH_E_UNSUPPORTED, "rotary: arrays must be fp32, bf16 or fp16");
+  TH_REQUIRE(d->batch > 0 && d->seq > 0 && d->heads > 0 && d->kv_heads >= 0,
+             "rotary: batch, seq and heads must be positive, kv_heads not negative");
+  TH_REQUIRE(d->head_dim > 0 && d->head_dim <= 1024, "rotary: head_dim must be 1..1024");
+  TH_REQUIRE(d->rotary_dim > 0 && d->rotary_dim % 2 == 0 && d->rotary_dim <= d->head_dim,
+             "rotary: rotary_dim must be even, positive and at most head_dim");
+  TH_REQUIRE(d->axes >= 1 && d->axes <= TH_ROTARY_AXES, "rotary: axes must be 1..4");
+  TH_REQUIRE((d->flags & ~(TH_ROTARY_PAIRS | TH_ROTARY_INVERSE)) == 0, "rotary: unknown flags");
+  TH_REQUIRE((int64_t)d->heads + d->kv_heads <= 65535, "rotary: heads and kv_heads must be at most 65535 together");
+  TH_REQUIRE(d->positions && d->freqs, "rotary: null positions or freqs");
+  const int half = d->rotary_dim / 2, size = d->dtype == TH_F32 ? 4 : 2;
+  RotaryArgs a{};
+  int sum = 0;
+  for (int i = 0; i < TH_ROTARY_AXES; ++i) {
+    if (i < d->axes) {
+      TH_REQUIRE(d->sections[i] >= 0 && d->sections[i] <= half, "rotary: sections must hold rotary_dim / 2 pairs together");
+      sum += d->sections[i];
+    }
+    a.ends[i] = i + 1 < d->axes ? sum : half;
+  }
+  TH_REQUIRE(sum == half, "rotary: sections must hold rotary_dim / 2 pairs together");
+  for (int64_t s : d->position_strides) TH_REQUIRE(s >= 0, "rotary: strides must not be negative");
+  if (int r = check_array(d->q, d->q_out, d->q_strides, d->q_out_strides, d, d->heads, size)) return r;
+  if (d->kv_heads)
+    if (int r = check_array(d->k, d->k_out, d->k_strides, d->k_out_strides, d, d->kv_heads, size)) return r;
+  a.a[0] = {d->q, d->q_out, d->q_strides[0], d->q_strides[1], d->q_strides[2],
+            d->q_out_strides[0], d->q_out_strides[1], d->q_out_strides[2], d->heads};
+  a.a[1] = {d->k, d->k_out, d->k_strides[0], d->k_strides[1], d->k_strides[2],
+            d->k_out_strides[0], d->k_out_strides[1], d->k_out_strides[2], d->kv_heads};
+  a.positions = d->positions, a.freqs = d->freqs;
+  a.pa = d->position_strides[0], a.ps = d->position_strides[1], a.pb = d->position_strides[2];
+  a.tokens = (int64_t)d->seq * d->batch;
+  a.seq = d->seq, a.half = half;
+  a.sign = d->flags & TH_ROTARY_INVERSE ? -1.0f : 1.0f;
+  // The widest vector (16 bytes at most) that divides a head's pairs and what passes.
+  const int pass = d->head_dim - d->rotary_dim;
+  int v = 16 / size;
+  while (half % v || pass % v) v /= 2;
+  const bool pairs = d->flags & TH_ROTARY_PAIRS;
+  const bool copy = pass && !(d->q_out == d->q && (!d->kv_heads || d->k_out == d->k));
+  a.turning = half / v, a.passing = copy ? pass / v : 0;
+  const int64_t per_token = (int64_t)(d->heads + d->kv_heads) * (a.turning + a.passing);
+  TH_REQUIRE(per_token <= (1 << 24), "rotary: heads * head_dim is too large");
+  // About four items a thread, at most 8 KB of angles.
+  a.per_block = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / per_token, 1024 / half));
+  const int64_t blocks = (a.tokens + a.per_block - 1) / a.per_block;
+  TH_REQUIRE(blocks <= 0xffffff, "rotary: batch * seq is too large");  // 2^32 threads
+  if (int r = th::require_ready()) return r;
+  const void* fn = d->dtype == TH_F32    ? kernel_of<TH_F32>(v, pairs)
+                   : d->dtype == TH_BF16 ? kernel_of<TH_BF16>(v, pairs)
+                                         : kernel_of<TH_F16>(v, pairs);
+  th::Builder b("rotary", 6);
+  const int k = b.kernel(fn, "rotary", dim3((unsigned)blocks), dim3(256), (uint32_t)(a.per_block * half * sizeof(float2)), a);
+  const size_t offs[6] = {TH_OFFSET(RotaryArgs, a),
+                          TH_OFFSET(RotaryArgs, a) + sizeof(RotaryArray),
+                          TH_OFFSET(RotaryArgs, a) + TH_OFFSET(RotaryArray, y),
+                          TH_OFFSET(RotaryArgs, a) + sizeof(RotaryArray) + TH_OFFSET(RotaryArray, y),
+                          TH_OFFSET(RotaryArgs, positions),
+                          TH_OFFSET(RotaryArgs, freqs)};
+  for (int i = 0; i < 6; ++i) b.ref(i, k, offs[i]);
+  const double n = (double)a.tokens * (d->heads + d->kv_heads);
+  b.work(2.0 * size * n * d->head_dim + 4.0 * a.tokens * d->axes, 6.0 * n * half, blocks);
+  *out = b.release();
+  return TH_OK;
+}
+
+}  // namespace
+
+extern "C" int th_build_rotary(const th_rotary_desc* d, th_launch** out) {
+  TH_REQUIRE(out != nullptr, "rotary: null result");
+  *out = nullptr;
+  return th::guarded([&] { return build(d, out); });
+}

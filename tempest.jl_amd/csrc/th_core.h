@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -30,6 +31,16 @@ int hip_fail(hipError_t e, const char* what);
   do {                                                             \
     if (!(cond)) return ::th::fail(TH_E_ARGUMENT, (msg));          \
   } while (0)
+
+// A C entry's body: an exception ends here, as TH_E_MEMORY.
+template <class F>
+int guarded(F&& body) {
+  try {
+    return body();
+  } catch (const std::exception& e) {
+    return fail(TH_E_MEMORY, e.what());
+  }
+}
 
 // ---- context ---------------------------------------------------------------
 
@@ -235,6 +246,9 @@ int build_attention_decode_fwd(const th_attention_desc* d, uint32_t align, bool 
 bool f32_attention_takes(const th_attention_desc* d);
 int build_attention_f32_fwd(const th_attention_desc* d, th_launch** out);
 int build_attention_f32_bwd(const th_attention_desc* d, th_launch** out);
+// Rows of `row` elements at these strides lie apart: ordered by stride, each
+// stride passes what the shorter ones span (cache.hip).  Extents of 1 need none.
+bool rows_apart(int64_t row, const int64_t* strides, const int64_t* extents, int n);
 // Products the bf16 tile kernel does not take (gemm_general.hip).
 int build_gemm_general(const th_gemm_desc* d, th_launch** out);
 

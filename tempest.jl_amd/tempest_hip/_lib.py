@@ -60,6 +60,38 @@ class AttentionDesc(ctypes.Structure):
                 ("kv_seq", c_i32), ("reserved", c_i32), ("starts", c_void_p), ("lengths", c_void_p)]
 
 
+class RotaryDesc(ctypes.Structure):
+    """th_rotary_desc (include/tempest_hip.h)."""
+    _fields_ = [("dtype", c_i32), ("batch", c_i32), ("seq", c_i32), ("heads", c_i32), ("kv_heads", c_i32),
+                ("head_dim", c_i32), ("rotary_dim", c_i32), ("axes", c_i32), ("sections", c_i32 * 4),
+                ("flags", c_i32), ("reserved", c_i32), ("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p),
+                ("k_out", c_void_p), ("q_strides", c_i64 * 3), ("k_strides", c_i64 * 3),
+                ("q_out_strides", c_i64 * 3), ("k_out_strides", c_i64 * 3), ("positions", c_void_p),
+                ("freqs", c_void_p), ("position_strides", c_i64 * 3)]
+
+
+class Cache(ctypes.Structure):
+    """th_cache (include/tempest_hip.h)."""
+    _fields_ = [("dtype", c_i32), ("heads", c_i32), ("head_dim", c_i32), ("page", c_i32), ("pages", c_i32),
+                ("reserved", c_i32), ("k", c_void_p), ("v", c_void_p), ("k_scales", c_void_p),
+                ("v_scales", c_void_p), ("strides", c_i64 * 3)]
+
+
+class CacheDesc(ctypes.Structure):
+    """th_cache_desc (include/tempest_hip.h)."""
+    _fields_ = [("cache", Cache), ("dtype", c_i32), ("batch", c_i32), ("seq", c_i32), ("table_pages", c_i32),
+                ("k", c_void_p), ("v", c_void_p), ("strides", c_i64 * 3), ("table", c_void_p),
+                ("lengths", c_void_p), ("counts", c_void_p)]
+
+
+class PagedDesc(ctypes.Structure):
+    """th_paged_desc (include/tempest_hip.h)."""
+    _fields_ = [("cache", Cache), ("dtype", c_i32), ("batch", c_i32), ("heads", c_i32), ("seq", c_i32),
+                ("table_pages", c_i32), ("causal", c_i32), ("window", c_i32), ("scale", c_f32), ("q", c_void_p),
+                ("o", c_void_p), ("lse", c_void_p), ("q_strides", c_i64 * 3), ("table", c_void_p),
+                ("lengths", c_void_p), ("counts", c_void_p)]
+
+
 class DeltaNetDesc(ctypes.Structure):
     """th_deltanet_desc (include/tempest_hip.h)."""
     _fields_ = [("batch", c_i32), ("heads", c_i32), ("seq", c_i32), ("dk", c_i32), ("dv", c_i32), ("chunk", c_i32),
@@ -172,6 +204,10 @@ SIGNATURES: dict[str, list] = {
     "th_gemm_tune": [P(GemmDesc), P(c_i32), P(c_i32), P(c_double)],
     "th_build_attention_fwd": [P(AttentionDesc), P(c_void_p)],
     "th_build_attention_bwd": [P(AttentionDesc), P(c_void_p)],
+    "th_build_rotary": [P(RotaryDesc), P(c_void_p)],
+    "th_build_cache_write": [P(CacheDesc), P(c_void_p)],
+    "th_build_cache_read": [P(CacheDesc), P(c_void_p)],
+    "th_build_attention_paged": [P(PagedDesc), P(c_void_p)],
     "th_build_deltanet_fwd": [P(DeltaNetDesc), P(c_void_p)],
     "th_build_deltanet": [P(DeltaNetDesc), P(c_void_p)],
     "th_build_floor": [P(FloorDesc), P(c_void_p)],

@@ -110,7 +110,7 @@ def tanh_layer_grad(d: int, h: int, c: int, w: int, b: int, x: int, loss: int, d
 
 # ---- op class (b) -----------------------------------------------------------
 
-F32, BF16, F16 = 0, 1, 4
+F32, BF16, F16, E4M3 = 0, 1, 4, 5  # TH_F32, ... (E4M3: a cache's)
 STORE, GELU, SQUARE_LOSS, GELU_BACKWARD = 0, 1, 2, 3
 F32_FACTORS, F16_FACTORS, ACCUMULATE, BF16X3 = 1, 2, 4, 8  # TH_GEMM_*
 # TH_TILE_*: which kernel and output tile a product runs on.
@@ -212,6 +212,110 @@ def attention_bwd(batch: int, heads: int, seq: int, q: int, k: int, v: int, o: i
                         scale=scale, flags=RECOMPUTE_DQ if recompute_dq else 0, **extra)
     return _built("th_build_attention_bwd",
                   ("q", "k", "v", "o", "lse", "dout", "dq", "dk", "dv", "starts", "lengths"), ctypes.byref(d))
+
+
+# ---- rotary positions -------------------------------------------------------
+
+ROTARY_PAIRS, ROTARY_INVERSE = 1, 2  # TH_ROTARY_*
+
+
+def _dense(head_dim: int, heads: int, seq: int) -> tuple[int, int, int]:
+    return (head_dim, heads * head_dim, seq * heads * head_dim)
+
+
+def rotary(batch: int, seq: int, heads: int, kv_heads: int, head_dim: int, q: int, k: int, q_out: int, k_out: int,
+           positions: int, freqs: int, sections=None, rotary_dim: int = 0, pairs: bool = False, inverse: bool = False,
+           dtype: int = BF16, q_strides=None, k_strides=None, q_out_strides=None, k_out_strides=None,
+           position_strides=None) -> Launch:
+    """q and k (d, heads, positions, batch) turned by their positions into q_out
+    and k_out (or in place): pair p by positions[axis(p)] * freqs[p], the first
+    rotary_dim features (0: all) in pairs half of that apart, or adjacent with
+    `pairs`; sections: the pairs of each axis (one axis by default); inverse:
+    turned back, the gradient.  positions int32 (axes, positions, batch), freqs
+    fp32.  kv_heads 0: q alone."""
+    rotary_dim = rotary_dim or head_dim
+    sections = list(sections) if sections is not None else [rotary_dim // 2]
+    axes = len(sections)
+    if axes > 4:
+        raise ValueError(f"rotary: at most 4 axes, got {axes}")
+    qs, ks = q_strides or _dense(head_dim, heads, seq), k_strides or _dense(head_dim, kv_heads, seq)
+    d = _lib.RotaryDesc(dtype=dtype, batch=batch, seq=seq, heads=heads, kv_heads=kv_heads, head_dim=head_dim,
+                        rotary_dim=rotary_dim, axes=axes, flags=(ROTARY_PAIRS if pairs else 0) |
+                        (ROTARY_INVERSE if inverse else 0), q=q, k=k or None, q_out=q_out, k_out=k_out or None,
+                        positions=positions, freqs=freqs)
+    d.sections[:axes] = sections
+    d.q_strides[:], d.k_strides[:] = list(qs), list(ks)
+    d.q_out_strides[:] = list(q_out_strides or (qs if q_out == q else _dense(head_dim, heads, seq)))
+    d.k_out_strides[:] = list(k_out_strides or (ks if k_out == k else _dense(head_dim, kv_heads, seq)))
+    d.position_strides[:] = list(position_strides or (1, axes, axes * seq))
+    return _built("th_build_rotary", ("q", "k", "q_out", "k_out", "positions", "freqs"), ctypes.byref(d))
+
+
+# ---- a key-value cache in pages ---------------------------------------------
+
+class Cache:
+    """A paged cache's arrays (th_cache): k and v (features, heads, positions in
+    a page, pages) of dtype BF16, F16 or E4M3 (then with k_scales and v_scales,
+    a byte each 32 features); strides along heads, positions and pages, by
+    default that order of memory.  The arrays stay the caller's."""
+
+    def __init__(self, k: int, v: int, heads: int, head_dim: int, page: int, pages: int, dtype: int = BF16,
+                 k_scales: int = 0, v_scales: int = 0, strides=None):
+        self.desc = _lib.Cache(dtype=dtype, heads=heads, head_dim=head_dim, page=page, pages=pages, k=k or None,
+                               v=v or None, k_scales=k_scales or None, v_scales=v_scales or None)
+        self.desc.strides[:] = list(strides or (head_dim, heads * head_dim, page * heads * head_dim))
+
+
+def _cache_desc(cache, batch, seq, k, v, table, lengths, table_pages, counts, dtype, strides):
+    c = cache.desc
+    if dtype is None:
+        dtype = BF16 if c.dtype == E4M3 else c.dtype
+    d = _lib.CacheDesc(cache=c, dtype=dtype, batch=batch, seq=seq, table_pages=table_pages, k=k, v=v, table=table,
+                       lengths=lengths, counts=counts or None)
+    d.strides[:] = list(strides or _dense(c.head_dim, c.heads, seq))
+    return d
+
+
+def cache_write(cache: Cache, batch: int, seq: int, k: int, v: int, table: int, lengths: int, table_pages: int,
+                counts: int = 0, dtype: int | None = None, strides=None) -> Launch:
+    """The new rows k and v (d, heads, positions, batch) into the cache's pages:
+    new position j < counts[b] (all seq without counts) of sequence b becomes
+    its position lengths[b] - counts[b] + j, in page table[that / page, b].
+    table int32 (table_pages, batch), lengths and counts int32 (batch); dtype of
+    k and v: the cache's, or BF16 or F16 for an E4M3 cache."""
+    return _built("th_build_cache_write",
+                  ("k", "v", "k_cache", "v_cache", "k_scales", "v_scales", "table", "lengths", "counts"),
+                  ctypes.byref(_cache_desc(cache, batch, seq, k, v, table, lengths, table_pages, counts, dtype,
+                                           strides)))
+
+
+def cache_read(cache: Cache, batch: int, seq: int, k: int, v: int, table: int, lengths: int, table_pages: int,
+               dtype: int | None = None, strides=None) -> Launch:
+    """The first min(lengths[b], seq) positions of each sequence back into k and v
+    (d, heads, positions, batch); the rows behind them stay as they are."""
+    return _built("th_build_cache_read",
+                  ("k", "v", "k_cache", "v_cache", "k_scales", "v_scales", "table", "lengths"),
+                  ctypes.byref(_cache_desc(cache, batch, seq, k, v, table, lengths, table_pages, 0, dtype, strides)))
+
+
+def attention_paged(cache: Cache, batch: int, heads: int, seq: int, q: int, o: int, table: int, lengths: int,
+                    table_pages: int, lse: int = 0, counts: int = 0, causal: bool = True, window: int = 0,
+                    scale: float = 0.0, dtype: int | None = None, q_strides=None) -> Launch:
+    """o = attention(q, the cache) for seq new positions a sequence, whose own
+    keys and values the cache holds already: query j of sequence b at position
+    lengths[b] - counts[b] + j sees the sequence's keys up to its own (all of
+    them with causal=False), with a window the last `window` of those.  lse
+    fp32; o and lse of rows j >= counts[b] stay as they are."""
+    c = cache.desc
+    if dtype is None:
+        dtype = BF16 if c.dtype == E4M3 else c.dtype
+    d = _lib.PagedDesc(cache=c, dtype=dtype, batch=batch, heads=heads, seq=seq, table_pages=table_pages,
+                       causal=int(causal), window=window, scale=scale, q=q, o=o, lse=lse or None, table=table,
+                       lengths=lengths, counts=counts or None)
+    d.q_strides[:] = list(q_strides or _dense(c.head_dim, heads, seq))
+    return _built("th_build_attention_paged",
+                  ("q", "o", "lse", "k_cache", "v_cache", "k_scales", "v_scales", "table", "lengths", "counts"),
+                  ctypes.byref(d))
 
 
 # ---- config 5 ---------------------------------------------------------------
