@@ -28,6 +28,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "attention_tiles.h"
 #include "cache.h"
@@ -126,22 +127,22 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// A sweep's keys: the table's row, or for pages in sixteens nothing else; the entries
-// in LDS from entry `first` on otherwise.
+// A sweep's keys: the table's row, its entries in LDS from entry `first` on
+// (pages not in sixteens), the last key, the head's bytes.
 struct Keys {
   const int32_t* table;
   const int32_t* entries;
-  int first, last;  // keys past `last` read the last again
-  int64_t at;       // the head's bytes
+  int first, last;
+  int64_t at;
 };
 
 typedef const __attribute__((address_space(4))) int32_t* constant_i32;
 
-// One block's operands in flight: K as A operands of key l % 16 of each half, V
-// as rows (features E (l % 16) + .. of keys 16 (j / 4) + 4 (l / 16) + j % 4).
-// A product's slot (g, e) is feature 32 s + 8 g + e for 16-bit K; for e4m3, so
-// that a lane's load is 16 bytes here too, slot (g, e) of products 2 s and 2 s + 1
-// are features 64 s + 16 g + e and + 8 + e.
+// One block's operands, in flight from load_k and load_v to the products: K as A operands
+// of key l % 16 of each half, V as rows (features E (l % 16) + .. of keys
+// 16 (j / 4) + 4 (l / 16) + j % 4).  A product's slot (g, e) is feature 32 s + 8 g +
+// e for 16-bit K; for e4m3, so that a lane's load is 16 bytes here too, slot
+// (g, e) of products 2 s and 2 s + 1 are features 64 s + 16 g + e and + 8 + e.
 // UNIFORM: pages in sixteens, so that each half block lies in one page.  The
 // wave reads its entry as a scalar, and the rows are at scalar addresses and
 // offsets that every block shares: no address is worked out on the vector ALU.
@@ -155,35 +156,15 @@ struct Block {
   u32x4 k[2][KL];
   uint32_t v[8][E / W];
   uint32_t scale[SW];  // key l % 32's: K's in lanes 0..31, V's in the others
-  uint32_t present;    // bit i: a page holds the block's key i
+
+  // Where a block's rows are: of each half its first (UNIFORM), in LDS otherwise.
+  struct Rows {
+    int64_t half[2];
+    uint32_t present;  // bit i: a page holds the block's key i
+  };
 
   __device__ __forceinline__ static int k_feature(int s, int g) {
     return CT == kE4m3 ? 64 * s + 16 * g : 32 * s + 8 * g;
-  }
-  __device__ __forceinline__ void load_k(const PagedArgs& p, int t, const char* row, int g) {
-#pragma unroll
-    for (int s = 0; s < KL; ++s) {
-      const int f = EXACT || k_feature(s, g) < p.head_dim ? k_feature(s, g) : 0;
-      k[t][s] = *reinterpret_cast<const u32x4*>(row + f * bytes);
-    }
-  }
-  __device__ __forceinline__ void load_v(const PagedArgs& p, int j, const char* row, int r) {
-    // Features come in eights, so the first of a lane's says for four or eight of them.
-#pragma unroll
-    for (int c = 0; c < (E + 7) / 8; ++c) {
-      const int f = EXACT || E * r + 8 * c < p.head_dim ? E * r + 8 * c : 0;
-      constexpr int words = (E < 8 ? E : 8) / W;
-      if constexpr (words == 4) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(row + f * bytes);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) v[j][4 * c + n] = x[n];
-      } else if constexpr (words == 2) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(row + f * bytes);
-        v[j][2 * c] = x[0], v[j][2 * c + 1] = x[1];
-      } else {
-        v[j][c] = *reinterpret_cast<const uint32_t*>(row + f * bytes);
-      }
-    }
   }
   __device__ __forceinline__ void load_scale(const PagedArgs& p, int64_t row) {
     if constexpr (CT == kE4m3) {
@@ -202,43 +183,71 @@ struct Block {
       }
     }
   }
-  __device__ __forceinline__ void load(const PagedArgs& p, const Keys& keys, WaveLds<D>& w, int key0) {
+  // K's operands and the scales of the block at key0 (whose first key is not past keys.last).
+  __device__ __forceinline__ Rows load_k(const PagedArgs& p, const Keys& keys, WaveLds<D>& w, int key0) {
     const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
+    Rows rows;
+    const char* row[2];
     if constexpr (UNIFORM) {
-      const char* base[2];  // of K's half t
-      int64_t row[2];
-      present = 0;
+      rows.present = 0;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         // A half past the last key: the last one's (its keys are seen by no row).
         const int key = min(key0 + 16 * t, keys.last & ~15), i = thd::quotient(key, p.pages.by_page);
         const int page = ((constant_i32)keys.table)[i];
         const bool found = (uint32_t)page < (uint32_t)p.pages.pages;
-        present |= found ? 0xffffu << 16 * t : 0u;
-        row[t] = (found ? page * p.pages.sg + (key - i * p.pages.page) * p.pages.sp : 0) * bytes + keys.at;
-        base[t] = p.k + row[t];
+        rows.present |= found ? 0xffffu << 16 * t : 0u;
+        rows.half[t] = (found ? page * p.pages.sg + (key - i * p.pages.page) * p.pages.sp : 0) * bytes + keys.at;
+        row[t] = p.k + rows.half[t] + (uint32_t)(r * ((int32_t)p.pages.sp * bytes));
       }
-      const int32_t sp = (int32_t)p.pages.sp * bytes;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) load_k(p, t, base[t] + (uint32_t)(r * sp), g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) load_v(p, j, p.v + row[j / 4] + (uint32_t)((4 * g + j % 4) * sp), r);
-      load_scale(p, (lane % kBlock < 16 ? row[0] : row[1]) + r * sp);
+      load_scale(p, (lane % kBlock < 16 ? rows.half[0] : rows.half[1]) + r * ((int32_t)p.pages.sp * bytes));
     } else {
-      const int key = min(key0 + lane % kBlock, keys.last);
+      const int key = min(key0 + lane % kBlock, keys.last);  // past the last the last again
       const int i = thd::quotient(key, p.pages.by_page);
       const int page = keys.entries[i - keys.first];
       const bool found = (uint32_t)page < (uint32_t)p.pages.pages;
       const int64_t mine = (found ? page * p.pages.sg + (key - i * p.pages.page) * p.pages.sp : 0) * bytes + keys.at;
-      present = (uint32_t)__ballot(found);
+      rows.half[0] = rows.half[1] = 0;
+      rows.present = (uint32_t)__ballot(found);
       if (lane < kBlock) w.row[lane] = mine;
       load_scale(p, mine);
       wave_fence();
 #pragma unroll
-      for (int t = 0; t < 2; ++t) load_k(p, t, p.k + w.row[16 * t + r], g);
+      for (int t = 0; t < 2; ++t) row[t] = p.k + w.row[16 * t + r];
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) load_v(p, j, p.v + w.row[16 * (j / 4) + 4 * g + j % 4], r);
-      wave_fence();
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < KL; ++s) {
+        const int f = EXACT || k_feature(s, g) < p.head_dim ? k_feature(s, g) : 0;
+        k[t][s] = *reinterpret_cast<const u32x4*>(row[t] + f * bytes);
+      }
+    return rows;
+  }
+  // V's rows of the block whose K was loaded last.
+  __device__ __forceinline__ void load_v(const PagedArgs& p, const Rows& rows, WaveLds<D>& w) {
+    const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const char* row = p.v;
+      if constexpr (UNIFORM) row += rows.half[j / 4] + (uint32_t)((4 * g + j % 4) * ((int32_t)p.pages.sp * bytes));
+      else row += w.row[16 * (j / 4) + 4 * g + j % 4];
+      // Features come in eights, so the first of a lane's says for four or eight of them.
+#pragma unroll
+      for (int c = 0; c < (E + 7) / 8; ++c) {
+        const int f = EXACT || E * r + 8 * c < p.head_dim ? E * r + 8 * c : 0;
+        constexpr int words = (E < 8 ? E : 8) / W;
+        if constexpr (words == 4) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(row + f * bytes);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) v[j][4 * c + n] = x[n];
+        } else if constexpr (words == 2) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(row + f * bytes);
+          v[j][2 * c] = x[0], v[j][2 * c + 1] = x[1];
+        } else {
+          v[j][c] = *reinterpret_cast<const uint32_t*>(row + f * bytes);
+        }
+      }
     }
   }
 };
@@ -305,10 +314,10 @@ __device__ __forceinline__ void split2_f16(float a, float b, uint32_t& w0, uint3
 
 // Whether one of a word's values is NaN or an infinity.
 template <int CT>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
   if constexpr (CT == kE4m3) {  // a byte of 0x7f but for its sign
     const uint32_t x = ~w & 0x7f7f7f7fu;
-    return (x - 0x01010101u) & ~x & 0x80808080u;
+    return ((x - 0x01010101u) & ~x & 0x80808080u) != 0;
   }
   constexpr uint32_t e = CT == kBf16 ? 0x7f80u : 0x7c00u;
   return (w & e) == e || (w >> 16 & e) == e;
@@ -386,10 +395,16 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_fwd(PagedArgs
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = f32x4{};
     float m = -INFINITY, l = 0.0f;
-    // The block of 32 keys from key0.
-    auto fold = [&](B& x, int key0) {
+    Keys keys{p.pages.table + (int64_t)p.pages.table_pages * b, entries, 0, last,
+              (int64_t)hk * p.pages.sh * B::bytes};
+    // The block of 32 keys from key0, the next one's loads (`more`) issued where its
+    // operands' registers are free: K's after this one's scores, V's after its sums.
+    B x;
+    typename B::Rows rows;
+    auto fold = [&](int key0, auto more) {
       Scales<D> sc;
       if constexpr (CT == kE4m3) sc.spread(waves[wave], x.scale, r, g);
+      const uint32_t present = rows.present;
       f32x4 s[2] = {f32x4{}, f32x4{}};
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
@@ -407,6 +422,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_fwd(PagedArgs
 #pragma unroll
           for (int y = QP - 1; y >= 0; --y) s[t] = product<kHalf>(a, qf[y][i], s[t]);
         }
+      if constexpr (more) rows = x.load_k(p, keys, waves[wave], key0 + kUnit);
+      __builtin_amdgcn_sched_barrier(0);
       // Adds V's weighted values to o; with `mask`, to the rows of position jj, the values that
       // it does not see taken as 0.
       u32x4 wp[WP];
@@ -441,20 +458,23 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_fwd(PagedArgs
       // times it is not 0.  What no row sees is taken as 0; where rows of several
       // positions differ in a value that is not finite, they go one position at a time.
       bool apart = false;
-      if (!(key0 >= all_lo && key0 + kBlock <= all_hi && x.present == 0xffffffffu)) {
-        bool strange = false;
+      if (!(key0 >= all_lo && key0 + kBlock <= all_hi && present == 0xffffffffu)) {
+        uint32_t strange = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int n = 16 * (i / 4) + 4 * g + i % 4, key = key0 + n;
-          const bool held = x.present >> n & 1, some = held && key >= first.lo && key < final.hi;
+          const bool held = present >> n & 1, some = held && key >= first.lo && key < final.hi;
           s[i / 4][i % 4] = held && key >= mine.lo && key < mine.hi ? s[i / 4][i % 4] : -INFINITY;
-          if constexpr (CT == kE4m3) sc.v[i] = some ? sc.v[i] : 1.0f;
+          const uint32_t keep = some ? 0xffffffffu : 0u, differ = key < all_lo || key >= all_hi ? 1u : 0u;
+          if constexpr (CT == kE4m3) {
+            sc.v[i] = some ? sc.v[i] : 1.0f;
+            strange |= differ & (sc.v[i] == INFINITY);
+          }
 #pragma unroll
           for (int d = 0; d < E / B::W; ++d) {
-            x.v[i][d] = some ? x.v[i][d] : 0u;
-            if (some && (key < all_lo || key >= all_hi)) strange |= not_finite<CT>(x.v[i][d]);
+            x.v[i][d] &= keep;
+            strange |= differ & not_finite<CT>(x.v[i][d]);
           }
-          if constexpr (CT == kE4m3) strange |= sc.v[i] == INFINITY;
         }
         apart = j1 > j0 && __any(strange);
       }
@@ -489,9 +509,9 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_fwd(PagedArgs
       if (!apart) weigh(false, 0);
       else
         for (int jj = j0; jj <= j1; ++jj) weigh(true, jj);
+      if constexpr (more) x.load_v(p, rows, waves[wave]);
+      __builtin_amdgcn_sched_barrier(0);
     };
-    Keys keys{p.pages.table + (int64_t)p.pages.table_pages * b, entries, 0, last,
-              (int64_t)hk * p.pages.sh * B::bytes};
     for (int s0 = k_lo, s1; s0 < k_hi; s0 = s1) {
       s1 = k_hi;
       if constexpr (!UNIFORM) {
@@ -506,18 +526,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_fwd(PagedArgs
       }
       int key0 = s0 + kBlock * wave;
       if (key0 < s1) {
-        B even, odd;
-        even.load(p, keys, waves[wave], key0);
-        while (true) {
-          if (key0 + kUnit < s1) odd.load(p, keys, waves[wave], key0 + kUnit);
-          fold(even, key0);
-          key0 += kUnit;
-          if (key0 >= s1) break;
-          if (key0 + kUnit < s1) even.load(p, keys, waves[wave], key0 + kUnit);
-          fold(odd, key0);
-          key0 += kUnit;
-          if (key0 >= s1) break;
-        }
+        rows = x.load_k(p, keys, waves[wave], key0);
+        x.load_v(p, rows, waves[wave]);
+        for (; key0 + kUnit < s1; key0 += kUnit) fold(key0, std::true_type{});
+        fold(key0, std::false_type{});
       }
     }
     l += __shfl_xor(l, 16, 64);
