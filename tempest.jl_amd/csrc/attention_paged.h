@@ -1,0 +1,854 @@
+// Op class (c), a cache in pages: attention forward for one or a few new
+// positions a sequence over K and V in pages (bf16, fp16, or e4m3 with a scale
+// of a power of two for each 32 features), head dims up to 256.
+//
+// The work is the cache's bytes: each (sequence, cache head) reads its K and V
+// once for the 16 query rows (position, head of the group) that are the columns of one
+// v_mfma_f32_16x16x32.
+//   - Only the device knows the lengths, so the workgroups divide the work
+//     there: the keys of all (sequence, head, 16 rows), in units of 128, lie in one
+//     line, of which each workgroup takes an equal piece, whatever the lengths and
+//     the table's room.  A piece that holds a whole sweep stores its result; the
+//     others leave partial results, two a workgroup at most, that a second kernel
+//     joins by their maxima and sums.
+//   - A wave takes 32 keys at a time, the next 32's K and V rows in flight in
+//     registers meanwhile.  The table's entries come from LDS, where they are
+//     laid once for many blocks: read from memory they would make each block wait for the
+//     loads before it, which come back in order.  32 lanes work out a row's
+//     address each and hand them on through LDS.
+//   - K rows are the A operand of S' = K Q', V rows transposed inside each lane
+//     (v_perm_b32) the A operand of O' += V' P', whose B operand the score
+//     registers are as they stand (keys 4 g + i and 16 + 4 g + i of lane group g
+//     being slots i and 4 + i).
+//   - The weights are fp32's: three bf16 parts (split2_towards0), or for fp16
+//     values two fp16 parts of 2^15 times the weight (22 bits, and 2^-39 of the
+//     largest weight where that is more), none of them 0 unless the weight is.
+//   - e4m3 becomes bf16 (v_cvt_scalef32_pk_bf16_fp8), exactly: 4 bits times a
+//     power of two; fp16 queries are then two bf16 parts, exactly.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <type_traits>
+
+#include "attention_tiles.h"
+#include "cache.h"
+
+namespace {
+
+using thd::u32x2_any;
+using thd::u32x4_any;
+typedef uint32_t u32_any __attribute__((aligned(1)));
+typedef uint16_t u16_any __attribute__((aligned(1)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kRows = 16;       // query rows a sweep holds
+constexpr int kBlock = 32;      // keys a wave takes at a time
+constexpr int kEntries = 2048;  // table entries in LDS at a time
+
+struct PagedArgs {
+  const uint16_t* q;
+  uint16_t* o;
+  float* lse;  // natural log, [b][s][h], or null
+  const char* k;
+  const char* v;
+  const uint8_t* ks;
+  const uint8_t* vs;
+  th::Pages pages;
+  float* part;      // unnormalised O of unfinished sweeps, [workgroup][first, last][row][D]
+  float* part_ml;   // and (m, l), [workgroup][first, last][row]
+  int32_t* pieces;  // of each sweep: the first piece's place in part, how many there are
+  int64_t q_sh, q_ss, q_sb;
+  int32_t seq, heads, kv_heads, batch, head_dim, causal, window;
+  int32_t group, tiles, sweeps;  // query heads a cache head; tiles of 16 rows; sweeps a sequence
+  int32_t workers;               // workgroups
+  th::Divisor by_group, by_tiles, by_sweeps, by_workers;
+  float scale;
+};
+
+// Keys [lo, hi) that new position j of a sequence sees (none where lo >= hi).
+struct Range {
+  int lo, hi;
+};
+__device__ __forceinline__ Range seen_by(const PagedArgs& p, int length, int count, int j) {
+  if (j >= count) return {0, 0};
+  if (!p.causal) return {0, length};
+  const int at = length - count + j;
+  return {p.window ? max(0, at - p.window + 1) : 0, at + 1};
+}
+
+// Sequence b's keys from the first that any new position sees, in blocks (fours of them,
+// so that a short sweep fills a workgroup's waves and shares none).
+struct Sequence {
+  int length, count, lo, blocks;
+};
+__device__ __forceinline__ Sequence sequence_of(const PagedArgs& p, int length, int count) {
+  const int lo = seen_by(p, length, count, 0).lo / kBlock * kBlock;
+  return {length, count, lo, count > 0 ? (length - lo + 4 * kBlock - 1) / (4 * kBlock) * 4 : 0};
+}
+__device__ __forceinline__ Sequence sequence_of(const PagedArgs& p, int b) {
+  return sequence_of(p, thd::length_of(p.pages, b), thd::count_of(p.pages, b, p.seq));
+}
+
+// x and all of the lanes' before.
+__device__ __forceinline__ int running_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr 1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);   // 2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);   // 4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);   // 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // rows 1, 3 + lane 15, 47's
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // rows 2, 3 + lane 31's
+  return x;
+}
+
+// The line of all sequences' blocks, sweep after sweep, and the piece of it that is this workgroup's:
+// 64 sequences at a time, a lane each.
+struct Line {
+  Sequence own;            // lane's: sequence b0 + lane
+  int end, b0;             // the line's length up to its end, from b0's start
+  int total, start, stop;  // the whole line; the piece
+  int b, before;           // a sequence, the line's length before it
+
+  __device__ __forceinline__ int step(const PagedArgs& p, int at) {
+    const int lane = threadIdx.x % 64;
+    b0 = at;
+    own = at + lane < p.batch ? sequence_of(p, at + lane) : Sequence{};
+    end = running_sum(own.blocks * p.sweeps);
+    return __builtin_amdgcn_readlane(end, 63);
+  }
+  __device__ __forceinline__ bool find(const PagedArgs& p, int least) {
+    total = 0;
+    for (int at = 0; at < p.batch; at += 64) total += step(p, at);
+    const int share = max(least, thd::quotient(total + p.workers - 1, p.by_workers));
+    start = blockIdx.x * share, stop = min(total, start + share);
+    if (start >= stop) return false;
+    before = 0;
+    if (p.batch > 64)
+      for (int at = 0;; at += 64) {
+        const int n = step(p, at);
+        if (before + n > start) break;
+        before += n;
+      }
+    const int at = __ffsll((unsigned long long)__ballot(before + end > start)) - 1;
+    b = b0 + at;
+    before += __builtin_amdgcn_readlane(end - own.blocks * p.sweeps, at);
+    return true;
+  }
+  // Sequence b, or one after it.
+  __device__ __forceinline__ Sequence sequence(const PagedArgs& p) const {
+    if (b - b0 >= 64) return sequence_of(p, b);
+    const int at = b - b0;
+    return {__builtin_amdgcn_readlane(own.length, at), __builtin_amdgcn_readlane(own.count, at),
+            __builtin_amdgcn_readlane(own.lo, at), __builtin_amdgcn_readlane(own.blocks, at)};
+  }
+};
+
+constexpr int kBf16 = 0, kF16 = 1, kE4m3 = 2;
+
+// What a wave shares with itself: where the block's rows are (bytes from the
+// arrays' start), and its scale bytes, K's 32 keys and then V's.
+template <int D>
+struct WaveLds {
+  int64_t row[kBlock];
+  uint32_t scale[(D + 127) / 128][2 * kBlock];
+};
+
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// A sweep's keys: the table's row, its entries in LDS from entry `first` on
+// (pages not in sixteens), the last key, the head's bytes.
+struct Keys {
+  const int32_t* table;
+  const int32_t* entries;
+  int first, last;
+  int64_t at;
+};
+
+typedef const __attribute__((address_space(4))) int32_t* constant_i32;
+
+// One block's operands, in flight from load_k and load_v to the products: K as A operands
+// of key l % 16 of each half, V as rows (features E (l % 16) + .. of keys
+// 16 (j / 4) + 4 (l / 16) + j % 4).  A product's slot (g, e) is feature 32 s + 8 g +
+// e for 16-bit K; for e4m3, so that a lane's load is 16 bytes here too, slot
+// (g, e) of products 2 s and 2 s + 1 are features 64 s + 16 g + e and + 8 + e.
+// UNIFORM: pages in sixteens, so that each half block lies in one page.  The
+// wave reads its entry as a scalar, and the rows are at scalar addresses and
+// offsets that every block shares: no address is worked out on the vector ALU.
+template <int D, int CT, bool EXACT, bool UNIFORM>
+struct Block {
+  static constexpr int E = D / 16;
+  static constexpr int bytes = CT == kE4m3 ? 1 : 2;
+  static constexpr int W = 4 / bytes;                        // features a word
+  static constexpr int KL = CT == kE4m3 ? D / 64 : D / 32;  // 16-byte pieces of a K row
+  static constexpr int SW = (D + 127) / 128;                 // words of scale bytes a key
+  u32x4 k[2][KL];
+  uint32_t v[8][E / W];
+  uint32_t scale[SW];  // key l % 32's: K's in lanes 0..31, V's in the others
+
+  // Where a block's rows are: of each half its first (UNIFORM), in LDS otherwise.
+  struct Rows {
+    int64_t half[2];
+    uint32_t present;  // bit i: a page holds the block's key i
+  };
+
+  __device__ __forceinline__ static int k_feature(int s, int g) {
+    return CT == kE4m3 ? 64 * s + 16 * g : 32 * s + 8 * g;
+  }
+  __device__ __forceinline__ void load_scale(const PagedArgs& p, int64_t row) {
+    if constexpr (CT == kE4m3) {
+      const uint8_t* from = (threadIdx.x % 64 < kBlock ? p.ks : p.vs) + row / 32;
+      if constexpr (!EXACT) {
+#pragma unroll
+        for (int c = 0; c < SW; ++c) scale[c] = 0;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+          if (32 * c < p.head_dim) scale[c / 4] |= (uint32_t)from[c] << (8 * (c % 4));
+      } else if constexpr (D == 64) {
+        scale[0] = *reinterpret_cast<const u16_any*>(from);
+      } else {
+#pragma unroll
+        for (int c = 0; c < SW; ++c) scale[c] = reinterpret_cast<const u32_any*>(from)[c];
+      }
+    }
+  }
+  // K's operands and the scales of the block at key0 (whose first key is not past keys.last).
+  __device__ __forceinline__ Rows load_k(const PagedArgs& p, const Keys& keys, WaveLds<D>& w, int key0) {
+    const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
+    Rows rows;
+    const char* row[2];
+    if constexpr (UNIFORM) {
+      rows.present = 0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        // A half past the last key: the last one's (its keys are seen by no row).
+        const int key = min(key0 + 16 * t, keys.last & ~15), i = thd::quotient(key, p.pages.by_page);
+        const int page = ((constant_i32)keys.table)[i];
+        const bool found = (uint32_t)page < (uint32_t)p.pages.pages;
+        rows.present |= found ? 0xffffu << 16 * t : 0u;
+        rows.half[t] = (found ? page * p.pages.sg + (key - i * p.pages.page) * p.pages.sp : 0) * bytes + keys.at;
+        row[t] = p.k + rows.half[t] + (uint32_t)(r * ((int32_t)p.pages.sp * bytes));
+      }
+      load_scale(p, (lane % kBlock < 16 ? rows.half[0] : rows.half[1]) + r * ((int32_t)p.pages.sp * bytes));
+    } else {
+      const int key = min(key0 + lane % kBlock, keys.last);  // past the last the last again
+      const int i = thd::quotient(key, p.pages.by_page);
+      const int page = keys.entries[i - keys.first];
+      const bool found = (uint32_t)page < (uint32_t)p.pages.pages;
+      const int64_t mine = (found ? page * p.pages.sg + (key - i * p.pages.page) * p.pages.sp : 0) * bytes + keys.at;
+      rows.half[0] = rows.half[1] = 0;
+      rows.present = (uint32_t)__ballot(found);
+      if (lane < kBlock) w.row[lane] = mine;
+      load_scale(p, mine);
+      wave_fence();
+#pragma unroll
+      for (int t = 0; t < 2; ++t) row[t] = p.k + w.row[16 * t + r];
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < KL; ++s) {
+        const int f = EXACT || k_feature(s, g) < p.head_dim ? k_feature(s, g) : 0;
+        k[t][s] = *reinterpret_cast<const u32x4*>(row[t] + f * bytes);
+      }
+    return rows;
+  }
+  // V's rows of the block whose K was loaded last.
+  __device__ __forceinline__ void load_v(const PagedArgs& p, const Rows& rows, WaveLds<D>& w) {
+    const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const char* row = p.v;
+      if constexpr (UNIFORM) row += rows.half[j / 4] + (uint32_t)((4 * g + j % 4) * ((int32_t)p.pages.sp * bytes));
+      else row += w.row[16 * (j / 4) + 4 * g + j % 4];
+      // Features come in eights, so the first of a lane's says for four or eight of them.
+#pragma unroll
+      for (int c = 0; c < (E + 7) / 8; ++c) {
+        const int f = EXACT || E * r + 8 * c < p.head_dim ? E * r + 8 * c : 0;
+        constexpr int words = (E < 8 ? E : 8) / W;
+        if constexpr (words == 4) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(row + f * bytes);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) v[j][4 * c + n] = x[n];
+        } else if constexpr (words == 2) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(row + f * bytes);
+          v[j][2 * c] = x[0], v[j][2 * c + 1] = x[1];
+        } else {
+          v[j][c] = *reinterpret_cast<const uint32_t*>(row + f * bytes);
+        }
+      }
+    }
+  }
+};
+
+// A block's scales as the operands need them: of K, a byte e << 23 for each half and 64
+// features; of V, one for each of the lane's keys.
+template <int D>
+struct Scales {
+  float k[2][D / 64], v[8];
+  __device__ __forceinline__ void spread(WaveLds<D>& w, const uint32_t* scale, int r, int g) {
+    const int lane = threadIdx.x % 64;
+    constexpr int SW = (D + 127) / 128;
+#pragma unroll
+    for (int c = 0; c < SW; ++c) w.scale[c][lane] = scale[c];
+    wave_fence();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < D / 64; ++s) {  // features 64 s + 16 g: block 2 s + g / 2
+        const uint32_t word = w.scale[s / 2][16 * t + r];
+        k[t][s] = __uint_as_float((word >> (16 * (s % 2) + 8 * (g / 2)) & 255u) << 23);
+      }
+    const int block = D / 16 * r / 32;  // of features E r
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32x4 words = *reinterpret_cast<const u32x4*>(&w.scale[block / 4][kBlock + 16 * h + 4 * g]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t word = words[i];
+        v[4 * h + i] = __uint_as_float((word >> (8 * (block % 4)) & 255u) << 23);
+      }
+    }
+    wave_fence();
+  }
+};
+
+__device__ __forceinline__ uint32_t bf16_of(uint32_t codes, float scale, int half) {
+  return __builtin_bit_cast(uint32_t, half ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
+}
+
+template <bool F16>
+__device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t rounded2(float a, float b) {
+  if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+  return pack2(a, b);
+}
+
+// x >= 0 (at most 2^15) in two fp16 parts, 22 bits or 2^-24, the first towards
+// 0 and neither 0 unless x is: an infinite value they multiply stays one.
+__device__ __forceinline__ void split2_f16(float a, float b, uint32_t& w0, uint32_t& w1) {
+  const float least = 5.9604645e-8f;  // fp16's least, 2^-24
+  const auto hi = __builtin_amdgcn_cvt_pkrtz(a > 0 ? fmaxf(a - least, least) : 0.0f, b > 0 ? fmaxf(b - least, least) : 0.0f);
+  const float ra = a > 0 ? fmaxf(a - (float)hi[0], least) : 0.0f, rb = b > 0 ? fmaxf(b - (float)hi[1], least) : 0.0f;
+  w0 = __builtin_bit_cast(uint32_t, hi);
+  w1 = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{ra, rb}, f16x2));
+}
+
+// Waves a SIMD that the registers are kept to.
+constexpr int waves_of(int D, bool SINGLE, bool WHOLE) {
+  if (WHOLE) return D > 64 ? 2 : 4;
+  return D > 128 ? 1 : D > 64 ? (SINGLE ? 3 : 2) : SINGLE ? 4 : 3;
+}
+
+// Whether one of a word's values is NaN or an infinity.
+template <int CT>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  if constexpr (CT == kE4m3) {  // a byte of 0x7f but for its sign
+    const uint32_t x = ~w & 0x7f7f7f7fu;
+    return ((x - 0x01010101u) & ~x & 0x80808080u) != 0;
+  }
+  constexpr uint32_t e = CT == kBf16 ? 0x7f80u : 0x7c00u;
+  return (w & e) == e || (w >> 16 & e) == e;
+}
+
+// A word with its values that are not finite as 0.
+template <int CT>
+__device__ __forceinline__ uint32_t finite_of(uint32_t w) {
+  if constexpr (CT == kE4m3) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) out |= (w >> i & 0x7fu) == 0x7fu ? 0u : w & 0xffu << i;
+    return out;
+  }
+  constexpr uint32_t e = CT == kBf16 ? 0x7f80u : 0x7c00u;
+  return ((w & e) == e ? 0u : w & 0xffffu) | ((w >> 16 & e) == e ? 0u : w & 0xffff0000u);
+}
+
+// EXACT: head_dim is D.  SINGLE: one new position a sequence.  WHOLE: a workgroup of
+// eight waves a sweep, no pieces and nothing to join.
+template <int D, int CT, bool F16, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE>
+__global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void paged_attn_fwd(PagedArgs p) {
+  constexpr int E = D / 16;  // features of V a lane holds of each key
+  constexpr int LD = D + 4;  // floats a row of a wave's O in LDS
+  constexpr int NW = WHOLE ? 8 : 4;               // waves
+  constexpr int kStep = kBlock * NW;              // keys they take at a time
+  constexpr bool kHalf = CT == kF16;              // products in fp16, not bf16
+  constexpr int QP = CT == kE4m3 && F16 ? 2 : 1;  // parts of q
+  constexpr int WP = kHalf ? 2 : 3;               // parts of a weight
+  constexpr float kBias = kHalf ? 15.0f : 0.0f;   // weights are held times 2^kBias
+  typedef Block<D, CT, EXACT, UNIFORM> B;
+  // LDS holds q's operands, what a wave shares with itself and the table's entries while a
+  // sweep runs, then the waves' results.
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  u32x4* qs = reinterpret_cast<u32x4*>(lds);  // [part][product][lane]
+  WaveLds<D>* waves = reinterpret_cast<WaveLds<D>*>(qs + QP * (D / 32) * 64);
+  int32_t* entries = reinterpret_cast<int32_t*>(waves + NW);
+  float(*Os)[kRows][LD] = reinterpret_cast<float(*)[kRows][LD]>(lds);
+  float(*Ms)[kRows] = reinterpret_cast<float(*)[kRows]>(Os + NW);
+  float(*Ls)[kRows] = Ms + NW;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
+  const float c = p.scale * kLog2e;
+  Line line;
+  if constexpr (WHOLE) {
+    line.b = thd::quotient(blockIdx.x, p.by_sweeps);
+    line.before = line.b * p.sweeps;
+    line.start = line.stop = 0;
+  } else {
+    if (!line.find(p, NW)) return;
+  }
+  for (int u = line.start; WHOLE || u < line.stop;) {
+    const int b = line.b;
+    int sweep, i0 = 0, i1, slot = -1;
+    Sequence seq;
+    if constexpr (WHOLE) {
+      seq = sequence_of(p, b);
+      sweep = blockIdx.x - line.before;
+      i1 = seq.blocks;
+    } else {
+      seq = line.sequence(p);
+      if (u - line.before >= seq.blocks * p.sweeps) {
+        line.before += seq.blocks * p.sweeps;
+        ++line.b;
+        continue;
+      }
+      sweep = (u - line.before) / seq.blocks, i0 = (u - line.before) - sweep * seq.blocks;
+      i1 = min(seq.blocks, i0 + line.stop - u);
+      const bool whole = i0 == 0 && i1 == seq.blocks;
+      slot = whole ? -1 : 2 * blockIdx.x + (u > line.start);
+      // Who has a sweep's first block says where its pieces are.
+      if (i0 == 0 && threadIdx.x == 0) {
+        const int share = max(NW, thd::quotient(line.total + p.workers - 1, p.by_workers));
+        int32_t* to = p.pieces + 2 * ((int64_t)b * p.sweeps + sweep);
+        to[0] = slot, to[1] = whole ? 0 : (u + seq.blocks - 1) / share - (int)blockIdx.x + 1;
+      }
+      u += i1 - i0;
+    }
+    const int hk = thd::quotient(sweep, p.by_tiles), tile = sweep - hk * p.tiles;
+    // The tile's rows are positions j0..j1 (position row / group, head row % group of the group).
+    const int length = seq.length, count = seq.count;
+    const int j0 = thd::quotient(kRows * tile, p.by_group);
+    if (WHOLE && j0 >= count) return;
+    const int j1 = thd::quotient(min(count * p.group, kRows * tile + kRows) - 1, p.by_group);
+    const Range first = seen_by(p, length, count, j0), final = seen_by(p, length, count, j1);
+    // Keys of this piece that any row sees, and those that every row sees.
+    const int k_lo = max(seq.lo + kBlock * i0, first.lo / kBlock * kBlock), k_hi = j0 < count ? min(seq.lo + kBlock * i1, final.hi) : 0;
+    const int all_lo = final.lo, all_hi = first.hi, last = final.hi - 1;
+    const int row = kRows * tile + r;
+    const bool live = row < count * p.group;
+    const int j = live ? thd::quotient(row, p.by_group) : j0, h = hk * p.group + (live ? row - j * p.group : 0);
+    const Range mine = live ? seen_by(p, length, count, j) : Range{0, 0};
+    if (!WHOLE) __syncthreads();  // (the sweep before's results are read)
+    const uint16_t* qrow = p.q + (int64_t)b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)j * p.q_ss;
+#pragma unroll
+    for (int s = wave; s < D / 32; s += NW) {
+      const int f = CT == kE4m3 ? B::k_feature(s / 2, g) + 8 * (s % 2) : B::k_feature(s, g);
+      const u32x4 x = live && (EXACT || f < p.head_dim) ? (u32x4) * reinterpret_cast<const u32x4_any*>(qrow + f) : u32x4{};
+      if constexpr (QP == 1) {
+        qs[64 * s + lane] = x;
+      } else {
+        u32x4 hi = {}, lo = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t word = x[i];  // (a bit cast of a vector's element itself takes element 0)
+          const f32x2 w = __builtin_convertvector(__builtin_bit_cast(f16x2, word), f32x2);
+          hi[i] = pack2(w[0], w[1]);
+          lo[i] = pack2(w[0] - __uint_as_float(hi[i] << 16), w[1] - __uint_as_float(hi[i] & 0xffff0000u));
+        }
+        qs[64 * s + lane] = hi, qs[64 * (D / 32 + s) + lane] = lo;
+      }
+    }
+    f32x4 o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = f32x4{};
+    float m = -INFINITY, l = 0.0f;
+    Keys keys{p.pages.table + (int64_t)p.pages.table_pages * b, entries, 0, last,
+              (int64_t)hk * p.pages.sh * B::bytes};
+    // The block of 32 keys from key0, the next one's loads (`more`) issued where its
+    // operands' registers are free: K's after this one's scores, V's after its sums.
+    B x;
+    typename B::Rows rows;
+    auto fold = [&](int key0, auto more) {
+      Scales<D> sc;
+      if constexpr (CT == kE4m3) sc.spread(waves[wave], x.scale, r, g);
+      const uint32_t present = rows.present;
+      f32x4 s[2] = {f32x4{}, f32x4{}};
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          u32x4 a;
+          if constexpr (CT == kE4m3) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) a[n] = bf16_of(x.k[t][i / 2][2 * (i % 2) + n / 2], sc.k[t][i / 2], n % 2);
+            if (!EXACT && B::k_feature(i / 2, g) >= p.head_dim) a = u32x4{};  // (loaded from feature 0)
+          } else {
+            a = x.k[t][i];
+            if (!EXACT && B::k_feature(i, g) >= p.head_dim) a = u32x4{};
+          }
+#pragma unroll
+          for (int y = QP - 1; y >= 0; --y) s[t] = product<kHalf>(a, qs[64 * (y * (D / 32) + i) + lane], s[t]);
+        }
+      if constexpr (more) rows = x.load_k(p, keys, waves[wave], key0 + kStep);
+      __builtin_amdgcn_sched_barrier(0);
+      // Where some row does not see some key, the value there may be anything, and 0
+      // times it is not 0.  What no row sees is taken as 0; of what rows of several
+      // positions differ in, values that are not finite are taken out and added to the rows that
+      // see them by themselves.
+      uint32_t differ = 0;  // bit i: some rows see the lane's key i, some do not
+      bool apart = false;
+      if (!(key0 >= all_lo && key0 + kBlock <= all_hi && present == 0xffffffffu)) {
+        uint32_t strange = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int n = 16 * (i / 4) + 4 * g + i % 4, key = key0 + n;
+          const bool held = present >> n & 1, some = held && key >= first.lo && key < final.hi;
+          s[i / 4][i % 4] = held && key >= mine.lo && key < mine.hi ? s[i / 4][i % 4] : -INFINITY;
+          if constexpr (CT == kE4m3) sc.v[i] = some ? sc.v[i] : 1.0f;
+          if constexpr (SINGLE) {
+#pragma unroll
+            for (int d = 0; d < E / B::W; ++d) x.v[i][d] &= some ? 0xffffffffu : 0u;
+            continue;
+          }
+          if (key < all_lo || key >= all_hi) differ |= 1u << i;
+#pragma unroll
+          for (int d = 0; d < E / B::W; ++d) {
+            x.v[i][d] &= some ? 0xffffffffu : 0u;
+            strange |= (differ >> i & 1) & not_finite<CT>(x.v[i][d]);
+          }
+          if constexpr (CT == kE4m3) strange |= (differ >> i & 1) & (sc.v[i] == INFINITY);
+        }
+        apart = !SINGLE && j1 > j0 && __any(strange != 0);
+      }
+      float mb = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mb = fmaxf(mb, s[i / 4][i % 4]);
+      mb = fmaxf(mb, __shfl_xor(mb, 16, 64));
+      mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
+      const float mn = fmaxf(m, mb * c);
+      const float shift = thd::lse_shift(mn);
+      if (__any(mn > m)) {  // (else every factor is 1)
+        const float alpha = __builtin_amdgcn_exp2f(m - shift);
+        l *= alpha;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= alpha;
+        m = mn;
+      }
+      u32x4 wp[WP];
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], c, kBias - shift));
+        l += w[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t a, b2, d2 = 0;
+        if constexpr (kHalf) split2_f16(w[2 * i], w[2 * i + 1], a, b2);
+        else split2_towards0(w[2 * i], w[2 * i + 1], a, b2, d2);
+        wp[0][i] = a, wp[1][i] = b2;
+        if constexpr (WP == 3) wp[2][i] = d2;
+      }
+      auto value = [&](int i, int d2) {  // features E (l % 16) + 2 d2 and + 1 of the lane's key i
+        if constexpr (CT == kE4m3) return bf16_of(x.v[i][d2 / 2], sc.v[i], d2 % 2);
+        else return x.v[i][d2];
+      };
+      if (apart) {
+        constexpr uint32_t one = kHalf ? 0x3c00u : 0x3f80u, top = kHalf ? 0x7c00u : 0x7f80u;
+        u32x4 sees;  // 1 for each key of the row's
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sees[i] = (w[2 * i] > 0 ? one : 0u) | (w[2 * i + 1] > 0 ? one << 16 : 0u);
+#pragma unroll
+        for (int d = 0; d < E; ++d)
+#pragma unroll 1
+          for (int kind = 0; kind < 3; ++kind) {  // infinity, -infinity, NaN
+            uint32_t is[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t y = value(i, d / 2) >> (16 * (d % 2)) & 0xffffu;
+              const bool that = kind == 2 ? (y & 0x7fffu) > top : y == (kind == 0 ? top : top | 0x8000u);
+              is[i] = that && (differ >> i & 1) ? one : 0u;
+            }
+            const u32x4 a = {is[0] | is[1] << 16, is[2] | is[3] << 16, is[4] | is[5] << 16, is[6] | is[7] << 16};
+            const f32x4 n = product<kHalf>(a, sees, f32x4{});
+            const float there = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[d][i] += n[i] > 0 ? there : 0.0f;
+          }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool whole = CT == kE4m3 && sc.v[i] == INFINITY;
+#pragma unroll
+          for (int d = 0; d < E / B::W; ++d)
+            if (differ >> i & 1) x.v[i][d] = whole ? 0u : finite_of<CT>(x.v[i][d]);
+          if (whole && (differ >> i & 1)) sc.v[i] = 1.0f;
+        }
+      }
+#pragma unroll
+      for (int d2 = 0; d2 < E / 2; ++d2) {
+        uint32_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = value(i, d2);
+        u32x4 even, odd;  // features E (l % 16) + 2 d2 and + 1 of the eight keys
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          even[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x05040100u);
+          odd[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x07060302u);
+        }
+#pragma unroll
+        for (int z = WP - 1; z >= 0; --z) {
+          o[2 * d2] = product<kHalf>(even, wp[z], o[2 * d2]);
+          o[2 * d2 + 1] = product<kHalf>(odd, wp[z], o[2 * d2 + 1]);
+        }
+      }
+      if constexpr (more) x.load_v(p, rows, waves[wave]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    for (int s0 = k_lo, s1; s0 < k_hi; s0 = s1) {
+      s1 = k_hi;
+      if constexpr (!UNIFORM) {
+        // As many whole units as the entries that fit in LDS reach.
+        keys.first = thd::quotient(s0, p.pages.by_page);
+        s1 = (int)min((int64_t)k_hi, s0 + ((int64_t)(keys.first + kEntries) * p.pages.page - s0) / kStep * kStep);
+        keys.last = min(last, s1 - 1);
+        const int n = thd::quotient(s1 - 1, p.pages.by_page) - keys.first + 1;
+        __syncthreads();  // (what was there is read)
+        for (int i = threadIdx.x; i < n; i += 64 * NW) entries[i] = keys.table[keys.first + i];
+        __syncthreads();
+      }
+      int key0 = s0 + kBlock * wave;
+      if (key0 < s1) {
+        rows = x.load_k(p, keys, waves[wave], key0);
+        x.load_v(p, rows, waves[wave]);
+      }
+      if constexpr (UNIFORM) __syncthreads();  // (q is there)
+      if (key0 < s1) {
+        for (; key0 + kStep < s1; key0 += kStep) fold(key0, std::true_type{});
+        fold(key0, std::false_type{});
+      }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    // Lane l holds row r's features E (4 g + i) + e in o[e][i].
+    __syncthreads();  // (no wave reads q any more)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<f32x4*>(&Os[wave][r][E * (4 * g + i) + e]) = f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
+    if (g == 0) Ms[wave][r] = m, Ls[wave][r] = l;
+    __syncthreads();
+    // The waves' parts in wave order: thread t takes row t / 16, features E (t % 16) + (0..E).
+    const int orow = threadIdx.x / 16, col = E * (threadIdx.x % 16), all = kRows * tile + orow;
+    if (threadIdx.x >= 256 || all >= count * p.group) {
+      if (WHOLE) return;
+      continue;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, Ms[w][orow]);
+    const float shift = thd::lse_shift(mx);
+    float sum = 0.0f;
+    f32x4 acc[E / 4] = {};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float a = __builtin_amdgcn_exp2f(Ms[w][orow] - shift);
+      sum += a * Ls[w][orow];
+#pragma unroll
+      for (int e = 0; e < E / 4; ++e) acc[e] += a * *reinterpret_cast<const f32x4*>(&Os[w][orow][col + 4 * e]);
+    }
+    if (slot >= 0) {
+      const int64_t to = (int64_t)slot * kRows + orow;
+#pragma unroll
+      for (int e = 0; e < E / 4; ++e) *reinterpret_cast<f32x4*>(p.part + to * D + col + 4 * e) = acc[e];
+      if (col == 0) reinterpret_cast<f32x2*>(p.part_ml)[to] = f32x2{mx - kBias, sum};
+      continue;
+    }
+    const int jo = thd::quotient(all, p.by_group), ho = hk * p.group + all - jo * p.group;
+    const float inv = mx == -INFINITY ? 0.0f : 1.0f / sum;
+    uint16_t* out = p.o + (int64_t)b * p.q_sb + (int64_t)ho * p.q_sh + (int64_t)jo * p.q_ss + col;
+#pragma unroll
+    for (int e = 0; e < E / 4; ++e)
+      if (EXACT || col + 4 * e < p.head_dim)
+        *reinterpret_cast<u32x2_any*>(out + 4 * e) =
+            u32x2{rounded2<F16>(acc[e][0] * inv, acc[e][1] * inv), rounded2<F16>(acc[e][2] * inv, acc[e][3] * inv)};
+    if (col == 0 && p.lse) p.lse[((int64_t)b * p.seq + jo) * p.heads + ho] = (mx - kBias + log2f(sum)) * kLn2;
+    if (WHOLE) return;
+  }
+}
+
+// The rows whose sweep lies in several pieces, or has no keys: a workgroup a row, its
+// threads in groups of D / 4, each of which takes every so manieth piece, four
+// loads at a time; then the groups' results in order.
+template <int D, bool F16>
+__global__ __launch_bounds__(1024) void paged_attn_join(PagedArgs p) {
+  constexpr int quads = D / 4;
+  __shared__ float Ms[1024 / quads], Ls[1024 / quads];
+  __shared__ f32x4 Os[1024];
+  const int h = blockIdx.x, pos = blockIdx.y, b = blockIdx.z;
+  const int hk = thd::quotient(h, p.by_group), row = pos * p.group + h - hk * p.group, tile = row / kRows;
+  const int32_t* pieces = p.pieces + 2 * ((int64_t)b * p.sweeps + hk * p.tiles + tile);
+  const int at0 = pieces[0], n = pieces[1];
+  const Sequence seq = sequence_of(p, b);
+  if (pos >= seq.count) return;
+  const int quad = threadIdx.x % quads, mine = threadIdx.x / quads, groups = blockDim.x / quads;
+  float m = -INFINITY, l = 0.0f;
+  f32x4 acc = {};
+  if (seq.blocks > 0) {
+    if (n == 0) return;  // stored already
+    for (int i0 = mine; i0 < n; i0 += 4 * groups) {
+      f32x2 x[4];
+      f32x4 y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // a piece past the last reads the last again, with no weight
+        const int piece = min(i0 + i * groups, n - 1);
+        // The first in either of its workgroup's places, the others in their first.
+        const int64_t from = (int64_t)(piece ? (at0 & ~1) + 2 * piece : at0) * kRows + row % kRows;
+        x[i] = reinterpret_cast<const f32x2*>(p.part_ml)[from];
+        y[i] = *reinterpret_cast<const f32x4*>(p.part + from * D + 4 * quad);
+      }
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mn = fmaxf(mn, x[i][0]);
+      const float shift = thd::lse_shift(mn), alpha = __builtin_amdgcn_exp2f(m - shift);
+      l *= alpha;
+      acc *= alpha;
+      m = mn;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i0 + i * groups < n) {
+          const float a = __builtin_amdgcn_exp2f(x[i][0] - shift);
+          l += a * x[i][1];
+          acc += a * y[i];
+        }
+    }
+    if (groups > 1) {
+      if (quad == 0) Ms[mine] = m, Ls[mine] = l;
+      Os[threadIdx.x] = acc;
+      __syncthreads();
+      if (mine > 0) return;
+      float mn = -INFINITY;
+      for (int i = 0; i < groups; ++i) mn = fmaxf(mn, Ms[i]);
+      const float shift = thd::lse_shift(mn);
+      l = 0.0f;
+      acc = f32x4{};
+      for (int i = 0; i < groups; ++i) {
+        const float a = __builtin_amdgcn_exp2f(Ms[i] - shift);
+        l += a * Ls[i];
+        acc += a * Os[i * quads + quad];
+      }
+      m = mn;
+    }
+  }
+  if (mine > 0) return;
+  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+  if (4 * quad < p.head_dim)
+    *reinterpret_cast<u32x2_any*>(p.o + b * p.q_sb + h * p.q_sh + pos * p.q_ss + 4 * quad) =
+        u32x2{rounded2<F16>(acc[0] * inv, acc[1] * inv), rounded2<F16>(acc[2] * inv, acc[3] * inv)};
+  if (quad == 0 && p.lse) p.lse[((int64_t)b * p.seq + pos) * p.heads + h] = (m + log2f(l)) * kLn2;
+}
+
+// Whether each sweep is one workgroup's.
+inline bool whole_sweeps(const th_paged_desc* d) {
+  int64_t keys = (int64_t)d->table_pages * d->cache.page;
+  if (d->window > 0) keys = std::min<int64_t>(keys, (int64_t)d->window + d->seq + 2 * kBlock);
+  return keys * (d->cache.head_dim + 32) <= (1 << 17);
+}
+
+template <int D, int CT, bool F16, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE>
+int launch(const th_paged_desc* d, th_launch** out) {
+  constexpr int NW = WHOLE ? 8 : 4;
+  constexpr size_t sweep_lds = (CT == kE4m3 && F16 ? 2 : 1) * kRows * D * 2 + NW * sizeof(WaveLds<D>) +
+                               (UNIFORM ? 0 : kEntries * sizeof(int32_t));
+  constexpr size_t result_lds = NW * kRows * (D + 4 + 2) * sizeof(float);
+  constexpr size_t lds = sweep_lds > result_lds ? sweep_lds : result_lds;
+  const void* fn = (const void*)paged_attn_fwd<D, CT, F16, EXACT, UNIFORM, SINGLE, WHOLE>;
+  if (lds > 65536) TH_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  const th_cache& cache = d->cache;
+  PagedArgs a{};
+  a.q = static_cast<const uint16_t*>(d->q), a.o = static_cast<uint16_t*>(d->o), a.lse = d->lse;
+  a.k = static_cast<const char*>(cache.k), a.v = static_cast<const char*>(cache.v);
+  a.ks = cache.k_scales, a.vs = cache.v_scales;
+  a.pages = th::pages_of(cache, d->table_pages, d->table, d->lengths, d->counts);
+  a.q_sh = d->q_strides[0], a.q_ss = d->q_strides[1], a.q_sb = d->q_strides[2];
+  a.seq = d->seq, a.heads = d->heads, a.kv_heads = cache.heads, a.batch = d->batch, a.head_dim = cache.head_dim;
+  a.causal = d->causal != 0, a.window = d->window;
+  a.scale = d->scale > 0 ? d->scale : 1.0f / sqrtf((float)cache.head_dim);
+  a.group = d->heads / cache.heads;
+  a.tiles = (int)(((int64_t)d->seq * a.group + kRows - 1) / kRows);
+  a.sweeps = a.tiles * cache.heads;
+  const int64_t keys = (int64_t)d->table_pages * cache.page, sweeps = (int64_t)a.sweeps * d->batch;
+  // As many workgroups as run at once, or as there are steps if that is fewer.
+  const int64_t resident = (int64_t)th::ctx().prop.multiProcessorCount * waves_of(D, SINGLE, WHOLE);
+  a.workers = WHOLE ? (int)sweeps : (int)std::min(resident, sweeps * ((keys + NW * kBlock - 1) / (NW * kBlock)));
+  a.by_group = th::divisor(a.group), a.by_tiles = th::divisor(a.tiles), a.by_sweeps = th::divisor(a.sweeps);
+  a.by_workers = th::divisor(a.workers);
+  th::Builder b("attention_paged", 10);
+  const int k = b.kernel(fn, WHOLE ? "paged_attn_fwd_whole" : "paged_attn_fwd", dim3(a.workers), dim3(64 * NW), (uint32_t)lds, a);
+  int end = k;
+  if (!WHOLE) {
+    // Threads for about as many pieces as a sweep has at the most.
+    int threads = 256;
+    while (threads < 1024 && threads / (D / 4) * 4 < a.workers / sweeps) threads *= 2;
+    end = b.kernel((const void*)paged_attn_join<D, F16>, "paged_attn_join", dim3(d->heads, d->seq, d->batch), dim3(threads), 0, a);
+    const uint64_t at_o = b.workspace((uint64_t)a.workers * 2 * kRows * D * sizeof(float));
+    const uint64_t at_ml = b.workspace((uint64_t)a.workers * 2 * kRows * 2 * sizeof(float));
+    const uint64_t at_pieces = b.workspace((uint64_t)sweeps * 2 * sizeof(int32_t));
+    for (int kk = k; kk <= end; ++kk) {
+      b.ws_ref(kk, TH_OFFSET(PagedArgs, part), at_o);
+      b.ws_ref(kk, TH_OFFSET(PagedArgs, part_ml), at_ml);
+      b.ws_ref(kk, TH_OFFSET(PagedArgs, pieces), at_pieces);
+    }
+  }
+  const size_t pages = TH_OFFSET(PagedArgs, pages);
+  const size_t offs[10] = {TH_OFFSET(PagedArgs, q),
+                           TH_OFFSET(PagedArgs, o),
+                           TH_OFFSET(PagedArgs, lse),
+                           TH_OFFSET(PagedArgs, k),
+                           TH_OFFSET(PagedArgs, v),
+                           TH_OFFSET(PagedArgs, ks),
+                           TH_OFFSET(PagedArgs, vs),
+                           pages + TH_OFFSET(th::Pages, table),
+                           pages + TH_OFFSET(th::Pages, lengths),
+                           pages + TH_OFFSET(th::Pages, counts)};
+  for (int v = 0; v < 10; ++v)
+    for (int kk = k; kk <= end; ++kk) b.ref(v, kk, offs[v]);
+  b.align(3, 16), b.align(4, 16);
+  // All the cache there is room for: how much is held only the device knows.
+  const double bytes = CT == kE4m3 ? 33.0 / 32 : 2, D0 = cache.head_dim, all = (double)d->batch * d->seq * d->heads;
+  b.work(2.0 * d->batch * cache.heads * (double)keys * D0 * bytes + 4.0 * all * D0, 4.0 * all * (double)keys * D0, a.workers);
+  *out = b.release();
+  return TH_OK;
+}
+
+template <int D, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE>
+int launch(const th_paged_desc* d, th_launch** out) {
+  if (d->cache.dtype == TH_BF16) return launch<D, kBf16, false, EXACT, UNIFORM, SINGLE, WHOLE>(d, out);
+  if (d->cache.dtype == TH_F16) return launch<D, kF16, true, EXACT, UNIFORM, SINGLE, WHOLE>(d, out);
+  return d->dtype == TH_F16 ? launch<D, kE4m3, true, EXACT, UNIFORM, SINGLE, WHOLE>(d, out)
+                            : launch<D, kE4m3, false, EXACT, UNIFORM, SINGLE, WHOLE>(d, out);
+}
+template <int D, bool EXACT, bool UNIFORM, bool SINGLE>
+int launch(const th_paged_desc* d, th_launch** out) {
+  return whole_sweeps(d) ? launch<D, EXACT, UNIFORM, SINGLE, true>(d, out) : launch<D, EXACT, UNIFORM, SINGLE, false>(d, out);
+}
+// Pages in sixteens (and rows of a half block within 31 bits) take the scalar addresses.
+template <int D>
+int launch_dim(const th_paged_desc* d, th_launch** out) {
+  if (d->cache.head_dim != D) return launch<D, false, false, false>(d, out);
+  if (d->cache.page % 16 != 0 || d->cache.strides[1] >= (1 << 26)) return launch<D, true, false, false>(d, out);
+  return d->seq > 1 ? launch<D, true, true, false>(d, out) : launch<D, true, true, true>(d, out);
+}
+
+}  // namespace

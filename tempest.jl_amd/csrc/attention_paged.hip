@@ -1,734 +1,14 @@
-// Op class (c), a cache in pages: attention forward for one or a few new
-// positions a sequence over K and V in pages (bf16, fp16, or e4m3 with a scale
-// of a power of two for each 32 features), head dims up to 256.
-//
-// The work is the cache's bytes: each (sequence, cache head) reads its K and V
-// once for the 16 query rows (position, head of the group) that are the columns of one
-// v_mfma_f32_16x16x32.
-//   - Only the device knows the lengths, so the workgroups divide the work
-//     there: the keys of all (sequence, head, 16 rows), in units of 128, lie in one
-//     line, of which each workgroup takes an equal piece, whatever the lengths and
-//     the table's room.  A piece that holds a whole sweep stores its result; the
-//     others leave partial results, two a workgroup at most, that a second kernel
-//     joins by their maxima and sums.
-//   - A wave takes 32 keys at a time, the next 32's K and V rows in flight in
-//     registers meanwhile.  The table's entries come from LDS, where they are
-//     laid once for many blocks: read from memory they would make each block wait for the
-//     loads before it, which come back in order.  32 lanes work out a row's
-//     address each and hand them on through LDS.
-//   - K rows are the A operand of S' = K Q', V rows transposed inside each lane
-//     (v_perm_b32) the A operand of O' += V' P', whose B operand the score
-//     registers are as they stand (keys 4 g + i and 16 + 4 g + i of lane group g
-//     being slots i and 4 + i).
-//   - The weights are fp32's: three bf16 parts (split2_towards0), or for fp16
-//     values two fp16 parts of 2^15 times the weight (22 bits, and 2^-39 of the
-//     largest weight where that is more), none of them 0 unless the weight is.
-//   - e4m3 becomes bf16 (v_cvt_scalef32_pk_bf16_fp8), exactly: 4 bits times a
-//     power of two; fp16 queries are then two bf16 parts, exactly.
-#include <hip/hip_runtime.h>
-
-#include <cmath>
-#include <type_traits>
-
-#include "attention_tiles.h"
+// Attention over a cache in pages: its checks.  The kernels are in
+// attention_paged.h, one unit for each of the head dims they are built for.
 #include "cache.h"
 
+namespace th {
+int paged_attention_64(const th_paged_desc* d, th_launch** out);
+int paged_attention_128(const th_paged_desc* d, th_launch** out);
+int paged_attention_256(const th_paged_desc* d, th_launch** out);
+}  // namespace th
+
 namespace {
-
-using thd::u32x2_any;
-using thd::u32x4_any;
-typedef uint32_t u32_any __attribute__((aligned(1)));
-typedef uint16_t u16_any __attribute__((aligned(1)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-
-constexpr int kRows = 16;       // query rows a sweep holds
-constexpr int kBlock = 32;      // keys a wave takes at a time
-constexpr int kUnit = 128;      // keys the four waves take at a time
-constexpr int kEntries = 2048;  // table entries in LDS at a time
-
-struct PagedArgs {
-  const uint16_t* q;
-  uint16_t* o;
-  float* lse;  // natural log, [b][s][h], or null
-  const char* k;
-  const char* v;
-  const uint8_t* ks;
-  const uint8_t* vs;
-  th::Pages pages;
-  float* part;     // unnormalised O of unfinished sweeps, [workgroup][first, last][row][D]
-  float* part_ml;  // and (m, l), [workgroup][first, last][row]
-  int64_t q_sh, q_ss, q_sb;
-  int32_t seq, heads, kv_heads, batch, head_dim, causal, window;
-  int32_t group, tiles;  // query heads a cache head; tiles of 16 rows
-  int32_t workers;       // workgroups
-  float scale;
-};
-
-// Keys [lo, hi) that new position j of a sequence sees (none where lo >= hi).
-struct Range {
-  int lo, hi;
-};
-__device__ __forceinline__ Range seen_by(const PagedArgs& p, int length, int count, int j) {
-  if (j >= count) return {0, 0};
-  if (!p.causal) return {0, length};
-  const int at = length - count + j;
-  return {p.window ? max(0, at - p.window + 1) : 0, at + 1};
-}
-
-// Sequence b's keys from the first that any new position sees, in units.
-struct Sequence {
-  int length, count, lo, units;
-};
-__device__ __forceinline__ Sequence sequence_of(const PagedArgs& p, int b) {
-  const int length = thd::length_of(p.pages, b), count = thd::count_of(p.pages, b, p.seq);
-  const int lo = seen_by(p, length, count, 0).lo / kBlock * kBlock;
-  return {length, count, lo, count > 0 ? (length - lo + kUnit - 1) / kUnit : 0};
-}
-
-// The sequence that holds unit `u` of the line (the first `before` units lie in
-// earlier ones), or with u < 0 the line's length: 64 sequences a step, a lane each.
-struct Place {
-  int b, before;
-};
-__device__ __forceinline__ Place place_of(const PagedArgs& p, int u) {
-  const int lane = threadIdx.x % 64, sweeps = p.kv_heads * p.tiles;
-  int before = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    const int own = b0 + lane < p.batch ? sequence_of(p, b0 + lane).units * sweeps : 0;
-    int end = own;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-      const int x = __shfl_up(end, o, 64);
-      if (lane >= o) end += x;
-    }
-    const uint64_t past = __ballot(before + end > u);
-    if (u >= 0 && past) {
-      const int at = __ffsll((unsigned long long)past) - 1;
-      return {b0 + at, before + __shfl(end - own, at, 64)};
-    }
-    before += __shfl(end, 63, 64);
-  }
-  return {p.batch, before};
-}
-
-constexpr int kBf16 = 0, kF16 = 1, kE4m3 = 2;
-
-// What a wave shares with itself: where the block's rows are (bytes from the
-// arrays' start), and its scale bytes, K's 32 keys and then V's.
-template <int D>
-struct WaveLds {
-  int64_t row[kBlock];
-  uint32_t scale[(D + 127) / 128][2 * kBlock];
-};
-
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
-// A sweep's keys: the table's row, its entries in LDS from entry `first` on
-// (pages not in sixteens), the last key, the head's bytes.
-struct Keys {
-  const int32_t* table;
-  const int32_t* entries;
-  int first, last;
-  int64_t at;
-};
-
-typedef const __attribute__((address_space(4))) int32_t* constant_i32;
-
-// One block's operands, in flight from load_k and load_v to the products: K as A operands
-// of key l % 16 of each half, V as rows (features E (l % 16) + .. of keys
-// 16 (j / 4) + 4 (l / 16) + j % 4).  A product's slot (g, e) is feature 32 s + 8 g +
-// e for 16-bit K; for e4m3, so that a lane's load is 16 bytes here too, slot
-// (g, e) of products 2 s and 2 s + 1 are features 64 s + 16 g + e and + 8 + e.
-// UNIFORM: pages in sixteens, so that each half block lies in one page.  The
-// wave reads its entry as a scalar, and the rows are at scalar addresses and
-// offsets that every block shares: no address is worked out on the vector ALU.
-template <int D, int CT, bool EXACT, bool UNIFORM>
-struct Block {
-  static constexpr int E = D / 16;
-  static constexpr int bytes = CT == kE4m3 ? 1 : 2;
-  static constexpr int W = 4 / bytes;                        // features a word
-  static constexpr int KL = CT == kE4m3 ? D / 64 : D / 32;  // 16-byte pieces of a K row
-  static constexpr int SW = (D + 127) / 128;                 // words of scale bytes a key
-  u32x4 k[2][KL];
-  uint32_t v[8][E / W];
-  uint32_t scale[SW];  // key l % 32's: K's in lanes 0..31, V's in the others
-
-  // Where a block's rows are: of each half its first (UNIFORM), in LDS otherwise.
-  struct Rows {
-    int64_t half[2];
-    uint32_t present;  // bit i: a page holds the block's key i
-  };
-
-  __device__ __forceinline__ static int k_feature(int s, int g) {
-    return CT == kE4m3 ? 64 * s + 16 * g : 32 * s + 8 * g;
-  }
-  __device__ __forceinline__ void load_scale(const PagedArgs& p, int64_t row) {
-    if constexpr (CT == kE4m3) {
-      const uint8_t* from = (threadIdx.x % 64 < kBlock ? p.ks : p.vs) + row / 32;
-      if constexpr (!EXACT) {
-#pragma unroll
-        for (int c = 0; c < SW; ++c) scale[c] = 0;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c)
-          if (32 * c < p.head_dim) scale[c / 4] |= (uint32_t)from[c] << (8 * (c % 4));
-      } else if constexpr (D == 64) {
-        scale[0] = *reinterpret_cast<const u16_any*>(from);
-      } else {
-#pragma unroll
-        for (int c = 0; c < SW; ++c) scale[c] = reinterpret_cast<const u32_any*>(from)[c];
-      }
-    }
-  }
-  // K's operands and the scales of the block at key0 (whose first key is not past keys.last).
-  __device__ __forceinline__ Rows load_k(const PagedArgs& p, const Keys& keys, WaveLds<D>& w, int key0) {
-    const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
-    Rows rows;
-    const char* row[2];
-    if constexpr (UNIFORM) {
-      rows.present = 0;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        // A half past the last key: the last one's (its keys are seen by no row).
-        const int key = min(key0 + 16 * t, keys.last & ~15), i = thd::quotient(key, p.pages.by_page);
-        const int page = ((constant_i32)keys.table)[i];
-        const bool found = (uint32_t)page < (uint32_t)p.pages.pages;
-        rows.present |= found ? 0xffffu << 16 * t : 0u;
-        rows.half[t] = (found ? page * p.pages.sg + (key - i * p.pages.page) * p.pages.sp : 0) * bytes + keys.at;
-        row[t] = p.k + rows.half[t] + (uint32_t)(r * ((int32_t)p.pages.sp * bytes));
-      }
-      load_scale(p, (lane % kBlock < 16 ? rows.half[0] : rows.half[1]) + r * ((int32_t)p.pages.sp * bytes));
-    } else {
-      const int key = min(key0 + lane % kBlock, keys.last);  // past the last the last again
-      const int i = thd::quotient(key, p.pages.by_page);
-      const int page = keys.entries[i - keys.first];
-      const bool found = (uint32_t)page < (uint32_t)p.pages.pages;
-      const int64_t mine = (found ? page * p.pages.sg + (key - i * p.pages.page) * p.pages.sp : 0) * bytes + keys.at;
-      rows.half[0] = rows.half[1] = 0;
-      rows.present = (uint32_t)__ballot(found);
-      if (lane < kBlock) w.row[lane] = mine;
-      load_scale(p, mine);
-      wave_fence();
-#pragma unroll
-      for (int t = 0; t < 2; ++t) row[t] = p.k + w.row[16 * t + r];
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int s = 0; s < KL; ++s) {
-        const int f = EXACT || k_feature(s, g) < p.head_dim ? k_feature(s, g) : 0;
-        k[t][s] = *reinterpret_cast<const u32x4*>(row[t] + f * bytes);
-      }
-    return rows;
-  }
-  // V's rows of the block whose K was loaded last.
-  __device__ __forceinline__ void load_v(const PagedArgs& p, const Rows& rows, WaveLds<D>& w) {
-    const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const char* row = p.v;
-      if constexpr (UNIFORM) row += rows.half[j / 4] + (uint32_t)((4 * g + j % 4) * ((int32_t)p.pages.sp * bytes));
-      else row += w.row[16 * (j / 4) + 4 * g + j % 4];
-      // Features come in eights, so the first of a lane's says for four or eight of them.
-#pragma unroll
-      for (int c = 0; c < (E + 7) / 8; ++c) {
-        const int f = EXACT || E * r + 8 * c < p.head_dim ? E * r + 8 * c : 0;
-        constexpr int words = (E < 8 ? E : 8) / W;
-        if constexpr (words == 4) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(row + f * bytes);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) v[j][4 * c + n] = x[n];
-        } else if constexpr (words == 2) {
-          const u32x2 x = *reinterpret_cast<const u32x2*>(row + f * bytes);
-          v[j][2 * c] = x[0], v[j][2 * c + 1] = x[1];
-        } else {
-          v[j][c] = *reinterpret_cast<const uint32_t*>(row + f * bytes);
-        }
-      }
-    }
-  }
-};
-
-// A block's scales as the operands need them: of K, a byte e << 23 for each half and 64
-// features; of V, one for each of the lane's keys.
-template <int D>
-struct Scales {
-  float k[2][D / 64], v[8];
-  __device__ __forceinline__ void spread(WaveLds<D>& w, const uint32_t* scale, int r, int g) {
-    const int lane = threadIdx.x % 64;
-    constexpr int SW = (D + 127) / 128;
-#pragma unroll
-    for (int c = 0; c < SW; ++c) w.scale[c][lane] = scale[c];
-    wave_fence();
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int s = 0; s < D / 64; ++s) {  // features 64 s + 16 g: block 2 s + g / 2
-        const uint32_t word = w.scale[s / 2][16 * t + r];
-        k[t][s] = __uint_as_float((word >> (16 * (s % 2) + 8 * (g / 2)) & 255u) << 23);
-      }
-    const int block = D / 16 * r / 32;  // of features E r
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const u32x4 words = *reinterpret_cast<const u32x4*>(&w.scale[block / 4][kBlock + 16 * h + 4 * g]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t word = words[i];
-        v[4 * h + i] = __uint_as_float((word >> (8 * (block % 4)) & 255u) << 23);
-      }
-    }
-    wave_fence();
-  }
-};
-
-__device__ __forceinline__ uint32_t bf16_of(uint32_t codes, float scale, int half) {
-  return __builtin_bit_cast(uint32_t, half ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true)
-                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
-}
-
-template <bool F16>
-__device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
-  if constexpr (F16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-template <bool F16>
-__device__ __forceinline__ uint32_t rounded2(float a, float b) {
-  if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
-  return pack2(a, b);
-}
-
-// x >= 0 (at most 2^15) in two fp16 parts, 22 bits or 2^-24, the first towards
-// 0 and neither 0 unless x is: an infinite value they multiply stays one.
-__device__ __forceinline__ void split2_f16(float a, float b, uint32_t& w0, uint32_t& w1) {
-  const float least = 5.9604645e-8f;  // fp16's least, 2^-24
-  const auto hi = __builtin_amdgcn_cvt_pkrtz(a > 0 ? fmaxf(a - least, least) : 0.0f, b > 0 ? fmaxf(b - least, least) : 0.0f);
-  const float ra = a > 0 ? fmaxf(a - (float)hi[0], least) : 0.0f, rb = b > 0 ? fmaxf(b - (float)hi[1], least) : 0.0f;
-  w0 = __builtin_bit_cast(uint32_t, hi);
-  w1 = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{ra, rb}, f16x2));
-}
-
-// Whether one of a word's values is NaN or an infinity.
-template <int CT>
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-  if constexpr (CT == kE4m3) {  // a byte of 0x7f but for its sign
-    const uint32_t x = ~w & 0x7f7f7f7fu;
-    return ((x - 0x01010101u) & ~x & 0x80808080u) != 0;
-  }
-  constexpr uint32_t e = CT == kBf16 ? 0x7f80u : 0x7c00u;
-  return (w & e) == e || (w >> 16 & e) == e;
-}
-
-template <int D, int CT, bool F16, bool EXACT, bool UNIFORM>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void paged_attn_fwd(PagedArgs p) {
-  constexpr int E = D / 16;  // features of V a lane holds of each key
-  constexpr int LD = D + 4;  // floats a row of a wave's O in LDS
-  constexpr bool kHalf = CT == kF16;              // products in fp16, not bf16
-  constexpr int QP = CT == kE4m3 && F16 ? 2 : 1;  // parts of q
-  constexpr int WP = kHalf ? 2 : 3;               // parts of a weight
-  constexpr float kBias = kHalf ? 15.0f : 0.0f;   // weights are held times 2^kBias
-  typedef Block<D, CT, EXACT, UNIFORM> B;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  float(*Os)[kRows][LD] = reinterpret_cast<float(*)[kRows][LD]>(lds);
-  float(*Ms)[kRows] = reinterpret_cast<float(*)[kRows]>(Os + 4);
-  float(*Ls)[kRows] = Ms + 4;
-  WaveLds<D>* waves = reinterpret_cast<WaveLds<D>*>(Ls + 4);
-  int32_t* entries = reinterpret_cast<int32_t*>(waves + 4);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
-  const int total = __builtin_amdgcn_readfirstlane(place_of(p, -1).before);
-  const int share = (total + p.workers - 1) / p.workers;
-  const int start = blockIdx.x * share, end = min(total, start + share);
-  if (start >= end) return;
-  const Place place = place_of(p, start);
-  int b = __builtin_amdgcn_readfirstlane(place.b), before = __builtin_amdgcn_readfirstlane(place.before);
-  const float c = p.scale * kLog2e;
-  for (int u = start; u < end;) {
-    const Sequence seq = sequence_of(p, b);
-    const int sweeps = p.kv_heads * p.tiles;
-    if (u - before >= seq.units * sweeps) {
-      before += seq.units * sweeps;
-      ++b;
-      continue;
-    }
-    const int sweep = (u - before) / seq.units, i0 = (u - before) - sweep * seq.units;
-    const int i1 = min(seq.units, i0 + end - u);
-    const int slot = i0 == 0 && i1 == seq.units ? -1 : u > start;
-    u += i1 - i0;
-    const int tile = sweep % p.tiles, hk = sweep / p.tiles;
-    // The tile's rows are positions j0..j1 (position row / group, head row % group of the group).
-    const int length = seq.length, count = seq.count;
-    const int j0 = kRows * tile / p.group, j1 = (min(count * p.group, kRows * tile + kRows) - 1) / p.group;
-    const Range first = seen_by(p, length, count, j0), final = seen_by(p, length, count, j1);
-    // Keys of this piece that any row sees, and those that every row sees.
-    const int k_lo = max(seq.lo + kUnit * i0, first.lo / kBlock * kBlock), k_hi = min(seq.lo + kUnit * i1, final.hi);
-    const int all_lo = final.lo, all_hi = first.hi, last = final.hi - 1;
-    const int row = kRows * tile + r;
-    const bool live = row < count * p.group;
-    const int j = live ? row / p.group : j0, h = hk * p.group + (live ? row % p.group : 0);
-    const Range mine = live ? seen_by(p, length, count, j) : Range{0, 0};
-    const uint16_t* qrow = p.q + (int64_t)b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)j * p.q_ss;
-    u32x4 qf[QP][D / 32];
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) {
-      const int f = CT == kE4m3 ? B::k_feature(s / 2, g) + 8 * (s % 2) : B::k_feature(s, g);
-      const bool there = live && (EXACT || f < p.head_dim);
-      const u32x4 x = there ? (u32x4) * reinterpret_cast<const u32x4_any*>(qrow + f) : u32x4{};
-      qf[0][s] = x;
-      if constexpr (QP == 2) {
-        u32x4 hi = {}, lo = {};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t word = x[i];  // (a bit cast of a vector's element itself takes element 0)
-          const f32x2 w = __builtin_convertvector(__builtin_bit_cast(f16x2, word), f32x2);
-          hi[i] = pack2(w[0], w[1]);
-          lo[i] = pack2(w[0] - __uint_as_float(hi[i] << 16), w[1] - __uint_as_float(hi[i] & 0xffff0000u));
-        }
-        qf[0][s] = hi, qf[1][s] = lo;
-      }
-    }
-    f32x4 o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = f32x4{};
-    float m = -INFINITY, l = 0.0f;
-    Keys keys{p.pages.table + (int64_t)p.pages.table_pages * b, entries, 0, last,
-              (int64_t)hk * p.pages.sh * B::bytes};
-    // The block of 32 keys from key0, the next one's loads (`more`) issued where its
-    // operands' registers are free: K's after this one's scores, V's after its sums.
-    B x;
-    typename B::Rows rows;
-    auto fold = [&](int key0, auto more) {
-      Scales<D> sc;
-      if constexpr (CT == kE4m3) sc.spread(waves[wave], x.scale, r, g);
-      const uint32_t present = rows.present;
-      f32x4 s[2] = {f32x4{}, f32x4{}};
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          u32x4 a;
-          if constexpr (CT == kE4m3) {
-#pragma unroll
-            for (int n = 0; n < 4; ++n) a[n] = bf16_of(x.k[t][i / 2][2 * (i % 2) + n / 2], sc.k[t][i / 2], n % 2);
-            if (!EXACT && B::k_feature(i / 2, g) >= p.head_dim) a = u32x4{};  // (loaded from feature 0)
-          } else {
-            a = x.k[t][i];
-            if (!EXACT && B::k_feature(i, g) >= p.head_dim) a = u32x4{};
-          }
-#pragma unroll
-          for (int y = QP - 1; y >= 0; --y) s[t] = product<kHalf>(a, qf[y][i], s[t]);
-        }
-      if constexpr (more) rows = x.load_k(p, keys, waves[wave], key0 + kUnit);
-      __builtin_amdgcn_sched_barrier(0);
-      // Adds V's weighted values to o; with `mask`, to the rows of position jj, the values that
-      // it does not see taken as 0.
-      u32x4 wp[WP];
-      auto weigh = [&](bool mask, int jj) {
-        const Range see = mask ? seen_by(p, length, count, jj) : Range{0, 0};
-#pragma unroll
-        for (int d2 = 0; d2 < E / 2; ++d2) {
-          uint32_t v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if constexpr (CT == kE4m3) v[i] = bf16_of(x.v[i][d2 / 2], sc.v[i], d2 % 2);
-            else v[i] = x.v[i][d2];
-            const int key = key0 + 16 * (i / 4) + 4 * g + i % 4;
-            if (mask) v[i] = key >= see.lo && key < see.hi ? v[i] : 0u;
-          }
-          u32x4 even, odd;  // features E (l % 16) + 2 d2 and + 1 of the eight keys
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            even[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x05040100u);
-            odd[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x07060302u);
-          }
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            f32x4 t = o[2 * d2 + y];
-#pragma unroll
-            for (int z = WP - 1; z >= 0; --z) t = product<kHalf>(y ? odd : even, wp[z], t);
-            o[2 * d2 + y] = !mask || j == jj ? t : o[2 * d2 + y];
-          }
-        }
-      };
-      // Where some row does not see some key, the value there may be anything, and 0
-      // times it is not 0.  What no row sees is taken as 0; where rows of several
-      // positions differ in a value that is not finite, they go one position at a time.
-      bool apart = false;
-      if (!(key0 >= all_lo && key0 + kBlock <= all_hi && present == 0xffffffffu)) {
-        uint32_t strange = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int n = 16 * (i / 4) + 4 * g + i % 4, key = key0 + n;
-          const bool held = present >> n & 1, some = held && key >= first.lo && key < final.hi;
-          s[i / 4][i % 4] = held && key >= mine.lo && key < mine.hi ? s[i / 4][i % 4] : -INFINITY;
-          const uint32_t keep = some ? 0xffffffffu : 0u, differ = key < all_lo || key >= all_hi ? 1u : 0u;
-          if constexpr (CT == kE4m3) {
-            sc.v[i] = some ? sc.v[i] : 1.0f;
-            strange |= differ & (sc.v[i] == INFINITY);
-          }
-#pragma unroll
-          for (int d = 0; d < E / B::W; ++d) {
-            x.v[i][d] &= keep;
-            strange |= differ & not_finite<CT>(x.v[i][d]);
-          }
-        }
-        apart = j1 > j0 && __any(strange);
-      }
-      float mb = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mb = fmaxf(mb, s[i / 4][i % 4]);
-      mb = fmaxf(mb, __shfl_xor(mb, 16, 64));
-      mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
-      const float mn = fmaxf(m, mb * c);
-      const float shift = thd::lse_shift(mn);
-      if (__any(mn > m)) {  // (else every factor is 1)
-        const float alpha = __builtin_amdgcn_exp2f(m - shift);
-        l *= alpha;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] *= alpha;
-        m = mn;
-      }
-      float w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], c, kBias - shift));
-        l += w[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t a, b2, d2 = 0;
-        if constexpr (kHalf) split2_f16(w[2 * i], w[2 * i + 1], a, b2);
-        else split2_towards0(w[2 * i], w[2 * i + 1], a, b2, d2);
-        wp[0][i] = a, wp[1][i] = b2;
-        if constexpr (WP == 3) wp[2][i] = d2;
-      }
-      if (!apart) weigh(false, 0);
-      else
-        for (int jj = j0; jj <= j1; ++jj) weigh(true, jj);
-      if constexpr (more) x.load_v(p, rows, waves[wave]);
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    for (int s0 = k_lo, s1; s0 < k_hi; s0 = s1) {
-      s1 = k_hi;
-      if constexpr (!UNIFORM) {
-        // As many whole units as the entries that fit in LDS reach.
-        keys.first = thd::quotient(s0, p.pages.by_page);
-        s1 = (int)min((int64_t)k_hi, s0 + ((int64_t)(keys.first + kEntries) * p.pages.page - s0) / kUnit * kUnit);
-        keys.last = min(last, s1 - 1);
-        const int n = thd::quotient(s1 - 1, p.pages.by_page) - keys.first + 1;
-        __syncthreads();  // (what was there is read)
-        for (int i = threadIdx.x; i < n; i += 256) entries[i] = keys.table[keys.first + i];
-        __syncthreads();
-      }
-      int key0 = s0 + kBlock * wave;
-      if (key0 < s1) {
-        rows = x.load_k(p, keys, waves[wave], key0);
-        x.load_v(p, rows, waves[wave]);
-        for (; key0 + kUnit < s1; key0 += kUnit) fold(key0, std::true_type{});
-        fold(key0, std::false_type{});
-      }
-    }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    // Lane l holds row r's features E (4 g + i) + e in o[e][i].
-    __syncthreads();  // (the sweep before's are read)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < E; e += 4)
-        *reinterpret_cast<f32x4*>(&Os[wave][r][E * (4 * g + i) + e]) = f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
-    if (g == 0) Ms[wave][r] = m, Ls[wave][r] = l;
-    __syncthreads();
-    // The four waves' parts in wave order: thread t takes row t / 16, features E (t % 16) + (0..E).
-    const int orow = threadIdx.x / 16, col = E * (threadIdx.x % 16), all = kRows * tile + orow;
-    if (all >= count * p.group) continue;
-    float mx = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, Ms[w][orow]);
-    const float shift = thd::lse_shift(mx);
-    float sum = 0.0f;
-    f32x4 acc[E / 4] = {};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float a = __builtin_amdgcn_exp2f(Ms[w][orow] - shift);
-      sum += a * Ls[w][orow];
-#pragma unroll
-      for (int e = 0; e < E / 4; ++e) acc[e] += a * *reinterpret_cast<const f32x4*>(&Os[w][orow][col + 4 * e]);
-    }
-    if (slot >= 0) {
-      const int64_t to = (2 * (int64_t)blockIdx.x + slot) * kRows + orow;
-#pragma unroll
-      for (int e = 0; e < E / 4; ++e) *reinterpret_cast<f32x4*>(p.part + to * D + col + 4 * e) = acc[e];
-      if (col == 0) reinterpret_cast<f32x2*>(p.part_ml)[to] = f32x2{mx - kBias, sum};
-      continue;
-    }
-    const int jo = all / p.group, ho = hk * p.group + all % p.group;
-    const float inv = mx == -INFINITY ? 0.0f : 1.0f / sum;
-    uint16_t* out = p.o + (int64_t)b * p.q_sb + (int64_t)ho * p.q_sh + (int64_t)jo * p.q_ss + col;
-#pragma unroll
-    for (int e = 0; e < E / 4; ++e)
-      if (EXACT || col + 4 * e < p.head_dim)
-        *reinterpret_cast<u32x2_any*>(out + 4 * e) =
-            u32x2{rounded2<F16>(acc[e][0] * inv, acc[e][1] * inv), rounded2<F16>(acc[e][2] * inv, acc[e][3] * inv)};
-    if (col == 0 && p.lse) p.lse[((int64_t)b * p.seq + jo) * p.heads + ho] = (mx - kBias + log2f(sum)) * kLn2;
-  }
-}
-
-// The rows whose sweep lies in several pieces, or in none: a workgroup a row, its
-// threads in groups of D / 4, each of which takes every so manieth piece, four
-// loads at a time; then the groups' results in order.
-template <int D, bool F16>
-__global__ void paged_attn_join(PagedArgs p) {
-  constexpr int quads = D / 4;
-  __shared__ float Ms[16], Ls[16];
-  __shared__ f32x4 Os[1024];
-  const int64_t at = blockIdx.x;  // [b][s][h]
-  const int h = (int)(at % p.heads), pos = (int)(at / p.heads % p.seq);
-  const int b = (int)(at / ((int64_t)p.heads * p.seq));
-  const Sequence seq = sequence_of(p, b);
-  if (pos >= seq.count) return;
-  const int hk = h / p.group, row = pos * p.group + h % p.group, tile = row / kRows;
-  const int quad = threadIdx.x % quads, mine = threadIdx.x / quads, groups = blockDim.x / quads;
-  float m = -INFINITY, l = 0.0f;
-  f32x4 acc = {};
-  if (seq.units > 0) {
-    int sum[2] = {0, 0};  // units before sequence b, and of all
-    for (int i = threadIdx.x % 64; i < p.batch; i += 64) {
-      const int n = sequence_of(p, i).units;
-      sum[0] += i < b ? n : 0, sum[1] += n;
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o /= 2) sum[0] += __shfl_xor(sum[0], o, 64), sum[1] += __shfl_xor(sum[1], o, 64);
-    const int sweeps = p.kv_heads * p.tiles;
-    const int share = (sum[1] * sweeps + p.workers - 1) / p.workers;
-    const int u0 = sum[0] * sweeps + (hk * p.tiles + tile) * seq.units, u1 = u0 + seq.units;
-    const int w0 = u0 / share, w1 = (u1 - 1) / share;
-    if (w0 == w1) return;  // stored already
-    const int64_t place = row % kRows;
-    for (int w = w0 + mine; w <= w1; w += 4 * groups) {
-      f32x2 x[4];
-      f32x4 y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // a piece past the last reads the last again, with no weight
-        const int at_w = min(w + i * groups, w1);
-        const int64_t from = (2 * (int64_t)at_w + (u0 > at_w * share)) * kRows + place;
-        x[i] = reinterpret_cast<const f32x2*>(p.part_ml)[from];
-        y[i] = *reinterpret_cast<const f32x4*>(p.part + from * D + 4 * quad);
-      }
-      float mn = m;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mn = fmaxf(mn, x[i][0]);
-      const float shift = thd::lse_shift(mn), alpha = __builtin_amdgcn_exp2f(m - shift);
-      l *= alpha;
-      acc *= alpha;
-      m = mn;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (w + i * groups <= w1) {
-          const float a = __builtin_amdgcn_exp2f(x[i][0] - shift);
-          l += a * x[i][1];
-          acc += a * y[i];
-        }
-    }
-    if (groups > 1) {
-      if (quad == 0) Ms[mine] = m, Ls[mine] = l;
-      Os[threadIdx.x] = acc;
-      __syncthreads();
-      if (mine > 0) return;
-      float mn = -INFINITY;
-      for (int i = 0; i < groups; ++i) mn = fmaxf(mn, Ms[i]);
-      const float shift = thd::lse_shift(mn);
-      l = 0.0f;
-      acc = f32x4{};
-      for (int i = 0; i < groups; ++i) {
-        const float a = __builtin_amdgcn_exp2f(Ms[i] - shift);
-        l += a * Ls[i];
-        acc += a * Os[i * quads + quad];
-      }
-      m = mn;
-    }
-  }
-  if (mine > 0) return;
-  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
-  if (4 * quad < p.head_dim)
-    *reinterpret_cast<u32x2_any*>(p.o + b * p.q_sb + h * p.q_sh + pos * p.q_ss + 4 * quad) =
-        u32x2{rounded2<F16>(acc[0] * inv, acc[1] * inv), rounded2<F16>(acc[2] * inv, acc[3] * inv)};
-  if (quad == 0 && p.lse) p.lse[at] = (m + log2f(l)) * kLn2;
-}
-
-template <int D, int CT, bool F16, bool EXACT, bool UNIFORM>
-int launch(const th_paged_desc* d, th_launch** out) {
-  constexpr size_t lds = (4 * kRows * (D + 4) + 8 * kRows) * sizeof(float) + 4 * sizeof(WaveLds<D>) + kEntries * sizeof(int32_t);
-  const void* fn = (const void*)paged_attn_fwd<D, CT, F16, EXACT, UNIFORM>;
-  if (lds > 65536) TH_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  const th_cache& cache = d->cache;
-  PagedArgs a{};
-  a.q = static_cast<const uint16_t*>(d->q), a.o = static_cast<uint16_t*>(d->o), a.lse = d->lse;
-  a.k = static_cast<const char*>(cache.k), a.v = static_cast<const char*>(cache.v);
-  a.ks = cache.k_scales, a.vs = cache.v_scales;
-  a.pages = th::pages_of(cache, d->table_pages, d->table, d->lengths, d->counts);
-  a.q_sh = d->q_strides[0], a.q_ss = d->q_strides[1], a.q_sb = d->q_strides[2];
-  a.seq = d->seq, a.heads = d->heads, a.kv_heads = cache.heads, a.batch = d->batch, a.head_dim = cache.head_dim;
-  a.causal = d->causal != 0, a.window = d->window;
-  a.scale = d->scale > 0 ? d->scale : 1.0f / sqrtf((float)cache.head_dim);
-  a.group = d->heads / cache.heads;
-  a.tiles = (int)(((int64_t)d->seq * a.group + kRows - 1) / kRows);
-  const int64_t keys = (int64_t)d->table_pages * cache.page;
-  const int64_t sweeps = (int64_t)a.tiles * cache.heads * d->batch;
-  // As many workgroups as run at once, or as there are units if that is fewer.
-  const int64_t resident = (int64_t)th::ctx().prop.multiProcessorCount * (D > 128 ? 1 : 2);
-  a.workers = (int)std::min(resident, sweeps * ((keys + kUnit - 1) / kUnit));
-  th::Builder b("attention_paged", 10);
-  const int k = b.kernel(fn, "paged_attn_fwd", dim3(a.workers), dim3(256), (uint32_t)lds, a);
-  // Threads for about as many pieces as a sweep has at the most.
-  int threads = 256;
-  while (threads < 1024 && threads / (D / 4) * 4 < a.workers / sweeps) threads *= 2;
-  const int64_t all = (int64_t)d->batch * d->seq * d->heads;
-  const int end = b.kernel((const void*)paged_attn_join<D, F16>, "paged_attn_join", dim3((unsigned)all), dim3(threads), 0, a);
-  const uint64_t at_o = b.workspace((uint64_t)a.workers * 2 * kRows * D * sizeof(float));
-  const uint64_t at_ml = b.workspace((uint64_t)a.workers * 2 * kRows * 2 * sizeof(float));
-  for (int kk = k; kk <= end; ++kk) {
-    b.ws_ref(kk, TH_OFFSET(PagedArgs, part), at_o);
-    b.ws_ref(kk, TH_OFFSET(PagedArgs, part_ml), at_ml);
-  }
-  const size_t pages = TH_OFFSET(PagedArgs, pages);
-  const size_t offs[10] = {TH_OFFSET(PagedArgs, q),
-                           TH_OFFSET(PagedArgs, o),
-                           TH_OFFSET(PagedArgs, lse),
-                           TH_OFFSET(PagedArgs, k),
-                           TH_OFFSET(PagedArgs, v),
-                           TH_OFFSET(PagedArgs, ks),
-                           TH_OFFSET(PagedArgs, vs),
-                           pages + TH_OFFSET(th::Pages, table),
-                           pages + TH_OFFSET(th::Pages, lengths),
-                           pages + TH_OFFSET(th::Pages, counts)};
-  for (int v = 0; v < 10; ++v)
-    for (int kk = k; kk <= end; ++kk) b.ref(v, kk, offs[v]);
-  b.align(3, 16), b.align(4, 16);
-  // All the cache there is room for: how much is held only the device knows.
-  const double bytes = CT == kE4m3 ? 33.0 / 32 : 2, D0 = cache.head_dim;
-  b.work(2.0 * d->batch * cache.heads * (double)keys * D0 * bytes + 4.0 * all * D0, 4.0 * all * (double)keys * D0, a.workers);
-  *out = b.release();
-  return TH_OK;
-}
-
-template <int D, bool EXACT, bool UNIFORM>
-int launch(const th_paged_desc* d, th_launch** out) {
-  if (d->cache.dtype == TH_BF16) return launch<D, kBf16, false, EXACT, UNIFORM>(d, out);
-  if (d->cache.dtype == TH_F16) return launch<D, kF16, true, EXACT, UNIFORM>(d, out);
-  return d->dtype == TH_F16 ? launch<D, kE4m3, true, EXACT, UNIFORM>(d, out)
-                            : launch<D, kE4m3, false, EXACT, UNIFORM>(d, out);
-}
-// Pages in sixteens (and rows of a half block within 31 bits) take the scalar addresses.
-template <int D, bool EXACT>
-int launch(const th_paged_desc* d, th_launch** out) {
-  return d->cache.page % 16 == 0 && d->cache.strides[1] < (1 << 26) ? launch<D, EXACT, true>(d, out)
-                                                                   : launch<D, EXACT, false>(d, out);
-}
 
 int build(const th_paged_desc* d, th_launch** out) {
   TH_REQUIRE(d != nullptr, "paged attention: null descriptor");
@@ -745,20 +25,16 @@ int build(const th_paged_desc* d, th_launch** out) {
   const int64_t extents[3] = {d->heads, d->seq, d->batch};
   TH_REQUIRE(th::rows_apart(d->cache.head_dim, d->q_strides, extents, 3), "paged attention: the rows of o overlap");
   TH_REQUIRE(d->table && d->lengths, "paged attention: null table or lengths");
+  TH_REQUIRE(d->heads <= 65535 && d->seq <= 65535, "paged attention: heads and seq must be at most 65535");
   const int64_t rows = (int64_t)d->seq * (d->heads / d->cache.heads);
-  const int64_t keys = (int64_t)d->table_pages * d->cache.page, sweeps = (rows + kRows - 1) / kRows * d->cache.heads * d->batch;
-  TH_REQUIRE(rows <= 0x7fffffff - kRows && (int64_t)d->batch * d->seq * d->heads <= (1 << 22),
+  const int64_t keys = (int64_t)d->table_pages * d->cache.page, sweeps = (rows + 15) / 16 * d->cache.heads * d->batch;
+  TH_REQUIRE(rows <= 0x7fffffff - 16 && (int64_t)d->batch * d->seq * d->heads <= (1 << 22),
              "paged attention: batch * seq * heads must be at most 2^22");
-  TH_REQUIRE((double)sweeps * (double)((keys + kUnit - 1) / kUnit) < 2147483647.0 - kRows * 65536,
+  TH_REQUIRE((double)sweeps * (double)((keys + 31) / 32) < 2147483647.0 - (1 << 20),
              "paged attention: the table's room for all heads is too large");
   if (int r = th::require_ready()) return r;
   const int n = d->cache.head_dim;
-  return n == 64    ? launch<64, true>(d, out)
-         : n == 128 ? launch<128, true>(d, out)
-         : n == 256 ? launch<256, true>(d, out)
-         : n < 64   ? launch<64, false>(d, out)
-         : n < 128  ? launch<128, false>(d, out)
-                    : launch<256, false>(d, out);
+  return n <= 64 ? th::paged_attention_64(d, out) : n <= 128 ? th::paged_attention_128(d, out) : th::paged_attention_256(d, out);
 }
 
 }  // namespace
