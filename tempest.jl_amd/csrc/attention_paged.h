@@ -172,20 +172,23 @@ struct Keys {
 typedef const __attribute__((address_space(4))) int32_t* constant_i32;
 
 // One block's operands, in flight from load_k and load_v to the products: K as A operands
-// of key l % 16 of each half, V as rows (features E (l % 16) + .. of keys
-// 16 (j / 4) + 4 (l / 16) + j % 4).  A product's slot (g, e) is feature 32 s + 8 g +
+// of key l % 16 of each half, V as rows (of keys 16 (j / 4) + 4 (l / 16) + j % 4, in
+// pieces of CH features, 16 bytes at the most, whole lines of memory a load: piece c from
+// feature CH (l % 16 + 16 c)).  A product's slot (g, e) is feature 32 s + 8 g +
 // e for 16-bit K; for e4m3, so that a lane's load is 16 bytes here too, slot
 // (g, e) of products 2 s and 2 s + 1 are features 64 s + 16 g + e and + 8 + e.
 // UNIFORM: pages in sixteens, so that each half block lies in one page.  The
 // wave reads its entry as a scalar, and the rows are at scalar addresses and
 // offsets that every block shares: no address is worked out on the vector ALU.
-template <int D, int CT, bool EXACT, bool UNIFORM>
+// STREAM: V's loads are non-temporal (K's lines are each read by two loads).
+template <int D, int CT, bool EXACT, bool UNIFORM, bool STREAM>
 struct Block {
   static constexpr int E = D / 16;
   static constexpr int bytes = CT == kE4m3 ? 1 : 2;
   static constexpr int W = 4 / bytes;                        // features a word
   static constexpr int KL = CT == kE4m3 ? D / 64 : D / 32;  // 16-byte pieces of a K row
   static constexpr int SW = (D + 127) / 128;                 // words of scale bytes a key
+  static constexpr int CH = E < 16 / bytes ? E : 16 / bytes; // features of V a load
   u32x4 k[2][KL];
   uint32_t v[8][E / W];
   uint32_t scale[SW];  // key l % 32's: K's in lanes 0..31, V's in the others
@@ -265,20 +268,19 @@ struct Block {
       const char* row = p.v;
       if constexpr (UNIFORM) row += rows.half[j / 4] + (uint32_t)((4 * g + j % 4) * ((int32_t)p.pages.sp * bytes));
       else row += w.row[16 * (j / 4) + 4 * g + j % 4];
-      // Features come in eights, so the first of a lane's says for four or eight of them.
+      // Features come in eights (e4m3 in 32s), so a piece's first says for all of it.
 #pragma unroll
-      for (int c = 0; c < (E + 7) / 8; ++c) {
-        const int f = EXACT || E * r + 8 * c < p.head_dim ? E * r + 8 * c : 0;
-        constexpr int words = (E < 8 ? E : 8) / W;
-        if constexpr (words == 4) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(row + f * bytes);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) v[j][4 * c + n] = x[n];
-        } else if constexpr (words == 2) {
-          const u32x2 x = *reinterpret_cast<const u32x2*>(row + f * bytes);
-          v[j][2 * c] = x[0], v[j][2 * c + 1] = x[1];
-        } else {
+      for (int c = 0; c < E / CH; ++c) {
+        const int f = EXACT || CH * (r + 16 * c) < p.head_dim ? CH * (r + 16 * c) : 0;
+        constexpr int words = CH / W;
+        if constexpr (words == 1) {
           v[j][c] = *reinterpret_cast<const uint32_t*>(row + f * bytes);
+        } else {
+          typedef uint32_t piece __attribute__((ext_vector_type(words)));
+          const piece* from = reinterpret_cast<const piece*>(row + f * bytes);
+          const piece x = STREAM ? __builtin_nontemporal_load(from) : *from;
+#pragma unroll
+          for (int n = 0; n < words; ++n) v[j][words * c + n] = x[n];
         }
       }
     }
@@ -303,7 +305,7 @@ struct Scales {
         const uint32_t word = w.scale[s / 2][16 * t + r];
         k[t][s] = __uint_as_float((word >> (16 * (s % 2) + 8 * (g / 2)) & 255u) << 23);
       }
-    const int block = D / 16 * r / 32;  // of features E r
+    const int block = D / 16 * r / 32;  // of features CH r
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const u32x4 words = *reinterpret_cast<const u32x4*>(&w.scale[block / 4][kBlock + 16 * h + 4 * g]);
@@ -375,7 +377,7 @@ __device__ __forceinline__ uint32_t finite_of(uint32_t w) {
   return ((w & e) == e ? 0u : w & 0xffffu) | ((w >> 16 & e) == e ? 0u : w & 0xffff0000u);
 }
 
-// EXACT: head_dim is D.  SINGLE: one new position a sequence.  WHOLE: a workgroup of
+// EXACT: head_dim is D.  SINGLE: one new position a sequence, in one tile.  WHOLE: a workgroup of
 // eight waves a sweep, no pieces and nothing to join.
 template <int D, int CT, bool F16, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE>
 __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void paged_attn_fwd(PagedArgs p) {
@@ -387,7 +389,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
   constexpr int QP = CT == kE4m3 && F16 ? 2 : 1;  // parts of q
   constexpr int WP = kHalf ? 2 : 3;               // parts of a weight
   constexpr float kBias = kHalf ? 15.0f : 0.0f;   // weights are held times 2^kBias
-  typedef Block<D, CT, EXACT, UNIFORM> B;
+  typedef Block<D, CT, EXACT, UNIFORM, SINGLE && !WHOLE> B;
   // LDS holds q's operands, what a wave shares with itself and the table's entries while a
   // sweep runs, then the waves' results.
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -560,7 +562,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
         wp[0][i] = a, wp[1][i] = b2;
         if constexpr (WP == 3) wp[2][i] = d2;
       }
-      auto value = [&](int i, int d2) {  // features E (l % 16) + 2 d2 and + 1 of the lane's key i
+      auto value = [&](int i, int d2) {  // features 2 d2 and 2 d2 + 1 of the lane's key i
         if constexpr (CT == kE4m3) return bf16_of(x.v[i][d2 / 2], sc.v[i], d2 % 2);
         else return x.v[i][d2];
       };
@@ -600,7 +602,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
         uint32_t v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = value(i, d2);
-        u32x4 even, odd;  // features E (l % 16) + 2 d2 and + 1 of the eight keys
+        u32x4 even, odd;  // the two features of the eight keys
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           even[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x05040100u);
@@ -640,13 +642,13 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    // Lane l holds row r's features E (4 g + i) + e in o[e][i].
+    // Lane l holds row r's features CH (4 g + i + 16 c) + e in o[CH c + e][i].
     __syncthreads();  // (no wave reads q any more)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < E; e += 4)
-        *reinterpret_cast<f32x4*>(&Os[wave][r][E * (4 * g + i) + e]) = f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
+        *reinterpret_cast<f32x4*>(&Os[wave][r][B::CH * (4 * g + i + 16 * (e / B::CH)) + e % B::CH]) = f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
     if (g == 0) Ms[wave][r] = m, Ls[wave][r] = l;
     __syncthreads();
     // The waves' parts in wave order: thread t takes row t / 16, features E (t % 16) + (0..E).
@@ -848,7 +850,8 @@ template <int D>
 int launch_dim(const th_paged_desc* d, th_launch** out) {
   if (d->cache.head_dim != D) return launch<D, false, false, false>(d, out);
   if (d->cache.page % 16 != 0 || d->cache.strides[1] >= (1 << 26)) return launch<D, true, false, false>(d, out);
-  return d->seq > 1 ? launch<D, true, true, false>(d, out) : launch<D, true, true, true>(d, out);
+  return d->seq > 1 || d->heads / d->cache.heads > kRows ? launch<D, true, true, false>(d, out)
+                                                         : launch<D, true, true, true>(d, out);
 }
 
 }  // namespace

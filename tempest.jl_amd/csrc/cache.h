@@ -13,18 +13,6 @@ namespace th {
 // What th_cache holds that a kernel can address, or TH_E_ARGUMENT / TH_E_UNSUPPORTED.
 int check_cache(const th_cache& c, int32_t dtype, int32_t table_pages, const char* what);
 
-// n / d for 0 <= n < 2^31 as (n * m) >> s: m = floor(2^s / d) + 1, s = 31 +
-// ceil(log2 d), so that m d exceeds 2^s by at most 2^(s - 31) and the quotient
-// by less than 1 / d.
-struct Divisor {
-  uint32_t m, s;
-};
-inline Divisor divisor(int32_t d) {
-  int l = 0;
-  while ((int64_t(1) << l) < d) ++l;
-  return {(uint32_t)((uint64_t(1) << (31 + l)) / (uint32_t)d + 1), (uint32_t)(31 + l)};
-}
-
 // Where a cache's rows are: element offsets, page by page.
 struct Pages {
   const int32_t* table;
@@ -46,10 +34,6 @@ namespace thd {
 
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
-
-__host__ __device__ __forceinline__ int quotient(int n, th::Divisor d) {
-  return (int)(((uint64_t)(uint32_t)n * d.m) >> d.s);
-}
 
 // Positions sequence b holds, and how many of them are new.
 __host__ __device__ __forceinline__ int length_of(const th::Pages& p, int b) {

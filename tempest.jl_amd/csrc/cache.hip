@@ -38,7 +38,8 @@ struct CacheArgs {
   th::Pages pages;
   int64_t sh, ss, sb;           // dense strides along heads, positions, batch
   int32_t seq, heads, chunks;   // chunks of 8 features a head
-  uint32_t items;               // chunks * heads * seq
+  int32_t items;                // chunks * heads * seq
+  th::Divisor by_heads, by_chunks;
 };
 
 template <bool F16>
@@ -99,14 +100,14 @@ __device__ __forceinline__ u32x4 values_of(u32x2 codes, float scale) {
 struct Item {
   int chunk, head, j;
 };
-__device__ __forceinline__ Item item_of(const CacheArgs& p, uint32_t i) {
-  const uint32_t row = i / (uint32_t)p.chunks, j = row / (uint32_t)p.heads;
-  return {(int)(i - row * p.chunks), (int)(row - j * p.heads), (int)j};
+__device__ __forceinline__ Item item_of(const CacheArgs& p, int i) {
+  const int row = thd::quotient(i, p.by_chunks), j = thd::quotient(row, p.by_heads);
+  return {i - row * p.chunks, row - j * p.heads, j};
 }
 
 template <bool E4M3, bool F16>
 __global__ __launch_bounds__(256) void cache_write(CacheArgs p) {
-  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  const int i = (int)(blockIdx.x * 256u + threadIdx.x);
   const int b = blockIdx.y;
   if (i >= p.items) return;
   const Item it = item_of(p, i);
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(256) void cache_write(CacheArgs p) {
 
 template <bool E4M3, bool F16>
 __global__ __launch_bounds__(256) void cache_read(CacheArgs p) {
-  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  const int i = (int)(blockIdx.x * 256u + threadIdx.x);
   const int b = blockIdx.y;
   if (i >= p.items) return;
   const Item it = item_of(p, i);
@@ -173,7 +174,7 @@ int build(const th_cache_desc* d, bool write, th_launch** out) {
   if (!write)
     TH_REQUIRE(th::rows_apart(c.head_dim, d->strides, extents, 3), "cache read: the rows of k (and of v) overlap");
   const int64_t items = (int64_t)c.head_dim / 8 * c.heads * d->seq;
-  TH_REQUIRE(items <= 0x7fffffff, std::string(what) + ": head_dim * heads * seq must be under 2^34");
+  TH_REQUIRE(items <= 0x7fffffff - 255, std::string(what) + ": head_dim * heads * seq must be under 2^34");
   if (int r = th::require_ready()) return r;
   CacheArgs a{};
   a.k = static_cast<uint16_t*>(d->k), a.v = static_cast<uint16_t*>(d->v);
@@ -182,7 +183,8 @@ int build(const th_cache_desc* d, bool write, th_launch** out) {
   a.pages = th::pages_of(c, d->table_pages, d->table, d->lengths, write ? d->counts : nullptr);
   a.sh = d->strides[0], a.ss = d->strides[1], a.sb = d->strides[2];
   a.seq = d->seq, a.heads = c.heads, a.chunks = c.head_dim / 8;
-  a.items = (uint32_t)items;
+  a.items = (int32_t)items;
+  a.by_heads = th::divisor(a.heads), a.by_chunks = th::divisor(a.chunks);
   const bool e = c.dtype == TH_E4M3, h = d->dtype == TH_F16;
   const void* fn = write ? (!e  ? (const void*)cache_write<false, false>
                             : h ? (const void*)cache_write<true, true>

@@ -30,11 +30,12 @@ struct RotaryArgs {
   const int32_t* positions;
   const float* freqs;
   int64_t pa, ps, pb;  // the positions' strides along axes, positions, batch
-  int64_t tokens;      // seq * batch
+  int32_t tokens;      // seq * batch
   int32_t seq, half;   // half: pairs a head
   int32_t ends[TH_ROTARY_AXES];  // pair p turns with the first axis whose end passes it
   int32_t turning, passing;      // items of a head: turned, copied
   int32_t per_block;             // tokens a workgroup
+  th::Divisor by_seq, by_half, by_token, by_head;  // (items of a token, of a head)
   float sign;
 };
 
@@ -90,50 +91,73 @@ __global__ __launch_bounds__(256) void rotary(RotaryArgs p) {
   typedef typename Element<T>::type E;
   typedef Vec<E, V> W;
   extern __shared__ float2 turns[];  // [token][pair]: sin, cos
-  const int64_t first = (int64_t)blockIdx.x * p.per_block;
-  const int tokens = (int)min((int64_t)p.per_block, p.tokens - first);
-  for (int i = threadIdx.x; i < tokens * p.half; i += 256) {
-    const int t = i / p.half, pair = i - t * p.half;
-    const int64_t token = first + t, b = token / p.seq, s = token - b * p.seq;
-    int axis = 0;
-#pragma unroll
-    for (int a = 0; a < TH_ROTARY_AXES - 1; ++a) axis += pair >= p.ends[a];
-    const int position = p.positions[axis * p.pa + s * p.ps + b * p.pb];
-    turns[i] = turned((double)position * ((double)p.freqs[pair] * 0.15915494309189535));
-  }
-  __syncthreads();
+  const int first = blockIdx.x * p.per_block, tokens = min(p.per_block, p.tokens - first);
   const int per_head = p.turning + p.passing;
-  const int per_token = (p.a[0].heads + p.a[1].heads) * per_head;
-  for (int i = threadIdx.x; i < tokens * per_token; i += 256) {
-    const int t = i / per_token, at = i - t * per_token;
-    int head = at / per_head;
-    const int item = at - head * per_head;
+  const int per_token = (p.a[0].heads + p.a[1].heads) * per_head, items = tokens * per_token;
+  // An item's place: its token of the workgroup's, its features of x and y.
+  struct Item {
+    const E* x;
+    E* y;
+    int t, item, f0, f1;
+  };
+  auto item_of = [&](int i) {
+    Item it;
+    it.t = thd::quotient(i, p.by_token);
+    const int at = i - it.t * per_token;
+    int head = thd::quotient(at, p.by_head);
+    it.item = at - head * per_head;
     const bool second = head >= p.a[0].heads;
     const RotaryArray& a = p.a[second];
     if (second) head -= p.a[0].heads;
-    const int64_t token = first + t, b = token / p.seq, s = token - b * p.seq;
-    const E* x = static_cast<const E*>(a.x) + head * a.xh + s * a.xs + b * a.xb;
-    E* y = static_cast<E*>(a.y) + head * a.yh + s * a.ys + b * a.yb;
-    if (item >= p.turning) {
-      const int f = 2 * p.half + V * (item - p.turning);
-      *reinterpret_cast<W*>(y + f) = *reinterpret_cast<const W*>(x + f);
-      continue;
-    }
-    const int f0 = PAIRS ? 2 * V * item : V * item, f1 = PAIRS ? f0 + V : f0 + p.half;
-    W u = *reinterpret_cast<const W*>(x + f0), v = *reinterpret_cast<const W*>(x + f1);
-    const float2* turn = turns + t * p.half + V * item;
+    const int token = first + it.t, b = thd::quotient(token, p.by_seq), s = token - b * p.seq;
+    it.x = static_cast<const E*>(a.x) + head * a.xh + (int64_t)s * a.xs + b * a.xb;
+    it.y = static_cast<E*>(a.y) + head * a.yh + s * a.ys + b * a.yb;
+    const bool turns = it.item < p.turning;
+    it.f0 = turns ? (PAIRS ? 2 * V * it.item : V * it.item) : 2 * p.half + V * (it.item - p.turning);
+    it.f1 = turns ? (PAIRS ? it.f0 + V : it.f0 + p.half) : it.f0;
+    return it;
+  };
+  // The first items are under way while the angles are formed.
+  Item it;
+  W u, v;
+  if ((int)threadIdx.x < items) {
+    it = item_of(threadIdx.x);
+    u = *reinterpret_cast<const W*>(it.x + it.f0), v = *reinterpret_cast<const W*>(it.x + it.f1);
+  }
+  for (int i = threadIdx.x; i < tokens * p.half; i += 256) {
+    const int t = thd::quotient(i, p.by_half), pair = i - t * p.half;
+    const int token = first + t, b = thd::quotient(token, p.by_seq), s = token - b * p.seq;
+    int axis = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      // Pair j: in halves element j of either, adjacent ones elements 2j and 2j + 1 of both together.
-      E& lo = PAIRS ? (2 * j < V ? u.x[2 * j] : v.x[2 * j - V]) : u.x[j];
-      E& hi = PAIRS ? (2 * j + 1 < V ? u.x[2 * j + 1] : v.x[2 * j + 1 - V]) : v.x[j];
-      const float sin = p.sign * turn[j].x, cos = turn[j].y;
-      const float g = wide<T>(lo), h = wide<T>(hi);
-      lo = narrow<T>(g * cos - h * sin);
-      hi = narrow<T>(g * sin + h * cos);
+    for (int a = 0; a < TH_ROTARY_AXES - 1; ++a) axis += pair >= p.ends[a];
+    const int position = p.positions[axis * p.pa + (int64_t)s * p.ps + b * p.pb];
+    turns[i] = turned((double)position * ((double)p.freqs[pair] * 0.15915494309189535));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < items;) {
+    const int next = i + 256;
+    Item it2;
+    W u2, v2;
+    if (next < items) {
+      it2 = item_of(next);
+      u2 = *reinterpret_cast<const W*>(it2.x + it2.f0), v2 = *reinterpret_cast<const W*>(it2.x + it2.f1);
     }
-    *reinterpret_cast<W*>(y + f0) = u;
-    *reinterpret_cast<W*>(y + f1) = v;
+    if (it.item < p.turning) {
+      const float2* turn = turns + it.t * p.half + V * it.item;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        // Pair j: in halves element j of either, adjacent ones elements 2j and 2j + 1 of both together.
+        E& lo = PAIRS ? (2 * j < V ? u.x[2 * j] : v.x[2 * j - V]) : u.x[j];
+        E& hi = PAIRS ? (2 * j + 1 < V ? u.x[2 * j + 1] : v.x[2 * j + 1 - V]) : v.x[j];
+        const float sin = p.sign * turn[j].x, cos = turn[j].y;
+        const float g = wide<T>(lo), h = wide<T>(hi);
+        lo = narrow<T>(g * cos - h * sin);
+        hi = narrow<T>(g * sin + h * cos);
+      }
+      *reinterpret_cast<W*>(it.y + it.f1) = v;
+    }
+    *reinterpret_cast<W*>(it.y + it.f0) = u;
+    it = it2, u = u2, v = v2, i = next;
   }
 }
 
@@ -195,7 +219,9 @@ int build(const th_rotary_desc* d, th_launch** out) {
             d->k_out_strides[0], d->k_out_strides[1], d->k_out_strides[2], d->kv_heads};
   a.positions = d->positions, a.freqs = d->freqs;
   a.pa = d->position_strides[0], a.ps = d->position_strides[1], a.pb = d->position_strides[2];
-  a.tokens = (int64_t)d->seq * d->batch;
+  const int64_t tokens = (int64_t)d->seq * d->batch;
+  TH_REQUIRE(tokens <= (1 << 30), "rotary: batch * seq must be at most 2^30");
+  a.tokens = (int32_t)tokens;
   a.seq = d->seq, a.half = half;
   a.sign = d->flags & TH_ROTARY_INVERSE ? -1.0f : 1.0f;
   // The widest vector (16 bytes at most) that divides a head's pairs and what passes.
@@ -209,9 +235,11 @@ int build(const th_rotary_desc* d, th_launch** out) {
   TH_REQUIRE(per_token <= (1 << 24), "rotary: heads * head_dim is too large");
   // About four items a thread, at most 8 KB of angles.
   a.per_block = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / per_token, 1024 / half));
-  const int64_t blocks = (a.tokens + a.per_block - 1) / a.per_block;
+  const int64_t blocks = (tokens + a.per_block - 1) / a.per_block;
   TH_REQUIRE(blocks <= 0xffffff, "rotary: batch * seq is too large");  // 2^32 threads
   if (int r = th::require_ready()) return r;
+  a.by_seq = th::divisor(a.seq), a.by_half = th::divisor(a.half), a.by_token = th::divisor((int)per_token);
+  a.by_head = th::divisor(a.turning + a.passing);
   const void* fn = d->dtype == TH_F32    ? kernel_of<TH_F32>(v, pairs)
                    : d->dtype == TH_BF16 ? kernel_of<TH_BF16>(v, pairs)
                                          : kernel_of<TH_F16>(v, pairs);

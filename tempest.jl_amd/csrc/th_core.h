@@ -246,6 +246,18 @@ int build_attention_decode_fwd(const th_attention_desc* d, uint32_t align, bool 
 bool f32_attention_takes(const th_attention_desc* d);
 int build_attention_f32_fwd(const th_attention_desc* d, th_launch** out);
 int build_attention_f32_bwd(const th_attention_desc* d, th_launch** out);
+// n / d for 0 <= n < 2^31 as (n * m) >> s: m = floor(2^s / d) + 1, s = 31 +
+// ceil(log2 d), so that m d exceeds 2^s by at most 2^(s - 31) and the quotient
+// by less than 1 / d.
+struct Divisor {
+  uint32_t m, s;
+};
+inline Divisor divisor(int32_t d) {
+  int l = 0;
+  while ((int64_t(1) << l) < d) ++l;
+  return {(uint32_t)((uint64_t(1) << (31 + l)) / (uint32_t)d + 1), (uint32_t)(31 + l)};
+}
+
 // Rows of `row` elements at these strides lie apart: ordered by stride, each
 // stride passes what the shorter ones span (cache.hip).  Extents of 1 need none.
 bool rows_apart(int64_t row, const int64_t* strides, const int64_t* extents, int n);
@@ -257,6 +269,10 @@ int build_gemm_general(const th_gemm_desc* d, th_launch** out);
 // ---- device helpers shared by kernels ---------------------------------------
 
 namespace thd {
+
+__host__ __device__ __forceinline__ int quotient(int n, th::Divisor d) {
+  return (int)(((uint64_t)(uint32_t)n * d.m) >> d.s);
+}
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
