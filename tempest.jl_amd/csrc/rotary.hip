@@ -34,6 +34,7 @@ struct RotaryArgs {
   int32_t seq, half;   // half: pairs a head
   int32_t ends[TH_ROTARY_AXES];  // pair p turns with the first axis whose end passes it
   int32_t turning, passing;      // items of a head: turned, copied
+  int32_t pass_second;           // features from a copied item's first vector to its second (0: it has one)
   int32_t per_block;             // tokens a workgroup
   th::Divisor by_seq, by_half, by_token, by_head;  // (items of a token, of a head)
   float sign;
@@ -80,11 +81,32 @@ __device__ __forceinline__ typename Element<T>::type narrow(float x) {
   if constexpr (T == TH_F16) return __builtin_bit_cast(uint16_t, (_Float16)x);
 }
 
-// V elements at the elements' own alignment.
+// V elements at the elements' own alignment, a load or a store (non-temporal:
+// 61 MB in 25 us, 29 with ordinary ones; non-temporal loads were slower where the arrays
+// had been in cache, 9.4 us for 7.6).
 template <class E, int V>
-struct __attribute__((packed, aligned(sizeof(E)))) Vec {
+struct Vec {
   E x[V];
 };
+template <int BYTES, int ALIGN>
+struct Words {
+  typedef uint32_t type __attribute__((ext_vector_type(BYTES / 4), aligned(ALIGN)));
+};
+template <int ALIGN>
+struct Words<2, ALIGN> {
+  typedef uint16_t type;
+};
+template <int V, class E>
+__device__ __forceinline__ Vec<E, V> load(const E* from) {
+  typedef typename Words<V * sizeof(E), sizeof(E)>::type words;
+  const words w = *reinterpret_cast<const words*>(from);
+  return __builtin_bit_cast(Vec<E, V>, w);
+}
+template <int V, class E>
+__device__ __forceinline__ void store(E* to, const Vec<E, V>& x) {
+  typedef typename Words<V * sizeof(E), sizeof(E)>::type words;
+  __builtin_nontemporal_store(__builtin_bit_cast(words, x), reinterpret_cast<words*>(to));
+}
 
 template <int T, int V, bool PAIRS>
 __global__ __launch_bounds__(256) void rotary(RotaryArgs p) {
@@ -100,29 +122,31 @@ __global__ __launch_bounds__(256) void rotary(RotaryArgs p) {
     E* y;
     int t, item, f0, f1;
   };
+  const RotaryArray qa = p.a[0], ka = p.a[1];
   auto item_of = [&](int i) {
     Item it;
     it.t = thd::quotient(i, p.by_token);
     const int at = i - it.t * per_token;
     int head = thd::quotient(at, p.by_head);
     it.item = at - head * per_head;
-    const bool second = head >= p.a[0].heads;
-    const RotaryArray& a = p.a[second];
-    if (second) head -= p.a[0].heads;
+    const bool second = head >= qa.heads;
+    auto of = [&](auto q, auto k) { return second ? k : q; };  // (scalars both, not loads from where the index says)
+    if (second) head -= qa.heads;
     const int token = first + it.t, b = thd::quotient(token, p.by_seq), s = token - b * p.seq;
-    it.x = static_cast<const E*>(a.x) + head * a.xh + (int64_t)s * a.xs + b * a.xb;
-    it.y = static_cast<E*>(a.y) + head * a.yh + s * a.ys + b * a.yb;
+    it.x = static_cast<const E*>(of(qa.x, ka.x)) + head * of(qa.xh, ka.xh) + s * of(qa.xs, ka.xs) + b * of(qa.xb, ka.xb);
+    it.y = static_cast<E*>(of(qa.y, ka.y)) + head * of(qa.yh, ka.yh) + s * of(qa.ys, ka.ys) + b * of(qa.yb, ka.yb);
     const bool turns = it.item < p.turning;
-    it.f0 = turns ? (PAIRS ? 2 * V * it.item : V * it.item) : 2 * p.half + V * (it.item - p.turning);
-    it.f1 = turns ? (PAIRS ? it.f0 + V : it.f0 + p.half) : it.f0;
+    it.f0 = turns ? (PAIRS ? 2 * V * it.item : V * it.item) : 2 * p.half + (V + p.pass_second) * (it.item - p.turning);
+    it.f1 = it.f0 + (turns ? (PAIRS ? V : p.half) : p.pass_second);
     return it;
   };
   // The first items are under way while the angles are formed.
   Item it;
   W u, v;
-  if ((int)threadIdx.x < items) {
-    it = item_of(threadIdx.x);
-    u = *reinterpret_cast<const W*>(it.x + it.f0), v = *reinterpret_cast<const W*>(it.x + it.f1);
+  const int step = 256 * gridDim.y, begin = 256 * blockIdx.y + threadIdx.x;
+  if (begin < items) {
+    it = item_of(begin);
+    u = load<V>(it.x + it.f0), v = load<V>(it.x + it.f1);
   }
   for (int i = threadIdx.x; i < tokens * p.half; i += 256) {
     const int t = thd::quotient(i, p.by_half), pair = i - t * p.half;
@@ -134,13 +158,13 @@ __global__ __launch_bounds__(256) void rotary(RotaryArgs p) {
     turns[i] = turned((double)position * ((double)p.freqs[pair] * 0.15915494309189535));
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < items;) {
-    const int next = i + 256;
+  for (int i = begin; i < items;) {
+    const int next = i + step;
     Item it2;
     W u2, v2;
     if (next < items) {
       it2 = item_of(next);
-      u2 = *reinterpret_cast<const W*>(it2.x + it2.f0), v2 = *reinterpret_cast<const W*>(it2.x + it2.f1);
+      u2 = load<V>(it2.x + it2.f0), v2 = load<V>(it2.x + it2.f1);
     }
     if (it.item < p.turning) {
       const float2* turn = turns + it.t * p.half + V * it.item;
@@ -154,9 +178,9 @@ __global__ __launch_bounds__(256) void rotary(RotaryArgs p) {
         lo = narrow<T>(g * cos - h * sin);
         hi = narrow<T>(g * sin + h * cos);
       }
-      *reinterpret_cast<W*>(it.y + it.f1) = v;
     }
-    *reinterpret_cast<W*>(it.y + it.f0) = u;
+    store(it.y + it.f0, u);
+    store(it.y + it.f1, v);
     it = it2, u = u2, v = v2, i = next;
   }
 }
@@ -230,7 +254,8 @@ int build(const th_rotary_desc* d, th_launch** out) {
   while (half % v || pass % v) v /= 2;
   const bool pairs = d->flags & TH_ROTARY_PAIRS;
   const bool copy = pass && !(d->q_out == d->q && (!d->kv_heads || d->k_out == d->k));
-  a.turning = half / v, a.passing = copy ? pass / v : 0;
+  a.turning = half / v, a.pass_second = pass % (2 * v) == 0 ? v : 0;
+  a.passing = copy ? pass / (v + a.pass_second) : 0;
   const int64_t per_token = (int64_t)(d->heads + d->kv_heads) * (a.turning + a.passing);
   TH_REQUIRE(per_token <= (1 << 24), "rotary: heads * head_dim is too large");
   // About four items a thread, at most 8 KB of angles.
@@ -243,8 +268,10 @@ int build(const th_rotary_desc* d, th_launch** out) {
   const void* fn = d->dtype == TH_F32    ? kernel_of<TH_F32>(v, pairs)
                    : d->dtype == TH_BF16 ? kernel_of<TH_BF16>(v, pairs)
                                          : kernel_of<TH_F16>(v, pairs);
+  // Few tokens: their items to several workgroups each.
+  const int64_t slices = blocks >= 512 ? 1 : std::min<int64_t>((a.per_block * per_token + 255) / 256, 512 / blocks);
   th::Builder b("rotary", 6);
-  const int k = b.kernel(fn, "rotary", dim3((unsigned)blocks), dim3(256), (uint32_t)(a.per_block * half * sizeof(float2)), a);
+  const int k = b.kernel(fn, "rotary", dim3((unsigned)blocks, (unsigned)slices), dim3(256), (uint32_t)(a.per_block * half * sizeof(float2)), a);
   const size_t offs[6] = {TH_OFFSET(RotaryArgs, a),
                           TH_OFFSET(RotaryArgs, a) + sizeof(RotaryArray),
                           TH_OFFSET(RotaryArgs, a) + TH_OFFSET(RotaryArray, y),
