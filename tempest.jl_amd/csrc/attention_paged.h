@@ -91,6 +91,12 @@ __device__ __forceinline__ Sequence sequence_of(const PagedArgs& p, int length, 
 __device__ __forceinline__ Sequence sequence_of(const PagedArgs& p, int b) {
   return sequence_of(p, thd::length_of(p.pages, b), thd::count_of(p.pages, b, p.seq));
 }
+// The same for a b that the wave shares, by scalar loads.
+typedef const __attribute__((address_space(4))) int32_t* constant_i32;
+__device__ __forceinline__ Sequence sequence_of_all(const PagedArgs& p, int b) {
+  const int length = min(max(((constant_i32)p.pages.lengths)[b], 0), p.pages.table_pages * p.pages.page);
+  return sequence_of(p, length, p.pages.counts ? min(max(((constant_i32)p.pages.counts)[b], 0), p.seq) : p.seq);
+}
 
 // x and all of the lanes' before.
 __device__ __forceinline__ int running_sum(int x) {
@@ -138,7 +144,7 @@ struct Line {
   }
   // Sequence b, or one after it.
   __device__ __forceinline__ Sequence sequence(const PagedArgs& p) const {
-    if (b - b0 >= 64) return sequence_of(p, b);
+    if (b - b0 >= 64) return sequence_of_all(p, b);
     const int at = b - b0;
     return {__builtin_amdgcn_readlane(own.length, at), __builtin_amdgcn_readlane(own.count, at),
             __builtin_amdgcn_readlane(own.lo, at), __builtin_amdgcn_readlane(own.blocks, at)};
@@ -155,6 +161,14 @@ struct WaveLds {
   uint32_t scale[(D + 127) / 128][2 * kBlock];
 };
 
+// The largest of the four lane groups' values, in each.
+__device__ __forceinline__ float max_of_groups(float x) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
 __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -168,8 +182,6 @@ struct Keys {
   int first, last;
   int64_t at;
 };
-
-typedef const __attribute__((address_space(4))) int32_t* constant_i32;
 
 // One block's operands, in flight from load_k and load_v to the products: K as A operands
 // of key l % 16 of each half, V as rows (of keys 16 (j / 4) + 4 (l / 16) + j % 4, in
@@ -193,7 +205,11 @@ struct Block {
   uint32_t v[8][E / W];
   uint32_t scale[SW];  // key l % 32's: K's in lanes 0..31, V's in the others
 
-  // Where a block's rows are: of each half its first (UNIFORM), in LDS otherwise.
+  // A block's table entries: of its halves (UNIFORM), of the lane's key l % 32.
+  struct Entries {
+    int page[2];
+  };
+  // Where its rows are: of each half its first (UNIFORM), in LDS otherwise.
   struct Rows {
     int64_t half[2];
     uint32_t present;  // bit i: a page holds the block's key i
@@ -219,30 +235,44 @@ struct Block {
       }
     }
   }
-  // K's operands and the scales of the block at key0 (whose first key is not past keys.last).
-  __device__ __forceinline__ Rows load_k(const PagedArgs& p, const Keys& keys, WaveLds<D>& w, int key0) {
+  // The block at key0's keys: past the last the last one again, a half past it the
+  // last one's (no row sees them).
+  __device__ __forceinline__ static int key_of(const Keys& keys, int key0, int t) {
+    return UNIFORM ? min(key0 + 16 * t, keys.last & ~15) : min(key0 + (int)(threadIdx.x % kBlock), keys.last);
+  }
+  __device__ __forceinline__ static Entries look(const PagedArgs& p, const Keys& keys, int key0) {
+    Entries e;
+#pragma unroll
+    for (int t = 0; t < (UNIFORM ? 2 : 1); ++t) {
+      const int i = thd::quotient(key_of(keys, key0, t), p.pages.by_page);
+      e.page[t] = UNIFORM ? ((constant_i32)keys.table)[i] : keys.entries[i - keys.first];
+    }
+    return e;
+  }
+  // K's operands and the scales of the block at key0, whose entries are `e`.
+  __device__ __forceinline__ Rows load_k(const PagedArgs& p, const Keys& keys, WaveLds<D>& w, const Entries& e, int key0) {
     const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
     Rows rows;
     const char* row[2];
+    // An entry that names no page: page 0's rows, which no row sees.
+    auto place = [&](int t, bool& found) {
+      const int key = key_of(keys, key0, t), at = key - thd::quotient(key, p.pages.by_page) * p.pages.page;
+      found = (uint32_t)e.page[t] < (uint32_t)p.pages.pages;
+      return ((found ? e.page[t] : 0) * p.pages.sg + at * p.pages.sp) * bytes + keys.at;
+    };
     if constexpr (UNIFORM) {
       rows.present = 0;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        // A half past the last key: the last one's (its keys are seen by no row).
-        const int key = min(key0 + 16 * t, keys.last & ~15), i = thd::quotient(key, p.pages.by_page);
-        const int page = ((constant_i32)keys.table)[i];
-        const bool found = (uint32_t)page < (uint32_t)p.pages.pages;
+        bool found;
+        rows.half[t] = place(t, found);
         rows.present |= found ? 0xffffu << 16 * t : 0u;
-        rows.half[t] = (found ? page * p.pages.sg + (key - i * p.pages.page) * p.pages.sp : 0) * bytes + keys.at;
         row[t] = p.k + rows.half[t] + (uint32_t)(r * ((int32_t)p.pages.sp * bytes));
       }
       load_scale(p, (lane % kBlock < 16 ? rows.half[0] : rows.half[1]) + r * ((int32_t)p.pages.sp * bytes));
     } else {
-      const int key = min(key0 + lane % kBlock, keys.last);  // past the last the last again
-      const int i = thd::quotient(key, p.pages.by_page);
-      const int page = keys.entries[i - keys.first];
-      const bool found = (uint32_t)page < (uint32_t)p.pages.pages;
-      const int64_t mine = (found ? page * p.pages.sg + (key - i * p.pages.page) * p.pages.sp : 0) * bytes + keys.at;
+      bool found;
+      const int64_t mine = place(0, found);
       rows.half[0] = rows.half[1] = 0;
       rows.present = (uint32_t)__ballot(found);
       if (lane < kBlock) w.row[lane] = mine;
@@ -415,7 +445,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
     int sweep, i0 = 0, i1, slot = -1;
     Sequence seq;
     if constexpr (WHOLE) {
-      seq = sequence_of(p, b);
+      seq = sequence_of_all(p, b);
       sweep = blockIdx.x - line.before;
       i1 = seq.blocks;
     } else {
@@ -451,26 +481,36 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
     const bool live = row < count * p.group;
     const int j = live ? thd::quotient(row, p.by_group) : j0, h = hk * p.group + (live ? row - j * p.group : 0);
     const Range mine = live ? seen_by(p, length, count, j) : Range{0, 0};
-    if (!WHOLE) __syncthreads();  // (the sweep before's results are read)
+    // q's operands, a product's to each wave in turn: on their way here, in LDS behind the
+    // first block's loads.
+    constexpr int QN = (D / 32 + NW - 1) / NW;
     const uint16_t* qrow = p.q + (int64_t)b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)j * p.q_ss;
+    u32x4 q[QN];
 #pragma unroll
-    for (int s = wave; s < D / 32; s += NW) {
-      const int f = CT == kE4m3 ? B::k_feature(s / 2, g) + 8 * (s % 2) : B::k_feature(s, g);
-      const u32x4 x = live && (EXACT || f < p.head_dim) ? (u32x4) * reinterpret_cast<const u32x4_any*>(qrow + f) : u32x4{};
-      if constexpr (QP == 1) {
-        qs[64 * s + lane] = x;
-      } else {
-        u32x4 hi = {}, lo = {};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t word = x[i];  // (a bit cast of a vector's element itself takes element 0)
-          const f32x2 w = __builtin_convertvector(__builtin_bit_cast(f16x2, word), f32x2);
-          hi[i] = pack2(w[0], w[1]);
-          lo[i] = pack2(w[0] - __uint_as_float(hi[i] << 16), w[1] - __uint_as_float(hi[i] & 0xffff0000u));
-        }
-        qs[64 * s + lane] = hi, qs[64 * (D / 32 + s) + lane] = lo;
-      }
+    for (int n = 0; n < QN; ++n) {
+      const int s = wave + NW * n, f = CT == kE4m3 ? B::k_feature(s / 2, g) + 8 * (s % 2) : B::k_feature(s, g);
+      q[n] = live && s < D / 32 && (EXACT || f < p.head_dim) ? (u32x4) * reinterpret_cast<const u32x4_any*>(qrow + f) : u32x4{};
     }
+    auto lay_q = [&]() {
+#pragma unroll
+      for (int n = 0; n < QN; ++n) {
+        const int s = wave + NW * n;
+        if (s >= D / 32) break;
+        if constexpr (QP == 1) {
+          qs[64 * s + lane] = q[n];
+        } else {
+          u32x4 hi = {}, lo = {};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t word = q[n][i];  // (a bit cast of a vector's element itself takes element 0)
+            const f32x2 w = __builtin_convertvector(__builtin_bit_cast(f16x2, word), f32x2);
+            hi[i] = pack2(w[0], w[1]);
+            lo[i] = pack2(w[0] - __uint_as_float(hi[i] << 16), w[1] - __uint_as_float(hi[i] & 0xffff0000u));
+          }
+          qs[64 * s + lane] = hi, qs[64 * (D / 32 + s) + lane] = lo;
+        }
+      }
+    };
     f32x4 o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = f32x4{};
@@ -481,6 +521,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
     // operands' registers are free: K's after this one's scores, V's after its sums.
     B x;
     typename B::Rows rows;
+    typename B::Entries next;  // the next block's entries
     auto fold = [&](int key0, auto more) {
       Scales<D> sc;
       if constexpr (CT == kE4m3) sc.spread(waves[wave], x.scale, r, g);
@@ -502,7 +543,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
 #pragma unroll
           for (int y = QP - 1; y >= 0; --y) s[t] = product<kHalf>(a, qs[64 * (y * (D / 32) + i) + lane], s[t]);
         }
-      if constexpr (more) rows = x.load_k(p, keys, waves[wave], key0 + kStep);
+      if constexpr (more) rows = x.load_k(p, keys, waves[wave], next, key0 + kStep);
       __builtin_amdgcn_sched_barrier(0);
       // Where some row does not see some key, the value there may be anything, and 0
       // times it is not 0.  What no row sees is taken as 0; of what rows of several
@@ -536,8 +577,9 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
       float mb = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; ++i) mb = fmaxf(mb, s[i / 4][i % 4]);
-      mb = fmaxf(mb, __shfl_xor(mb, 16, 64));
-      mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
+      mb = max_of_groups(mb);
+      // (behind the scores: nothing waits for LDS until they are here)
+      if constexpr (more) next = B::look(p, keys, key0 + 2 * kStep);
       const float mn = fmaxf(m, mb * c);
       const float shift = thd::lse_shift(mn);
       if (__any(mn > m)) {  // (else every factor is 1)
@@ -617,27 +659,40 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
       if constexpr (more) x.load_v(p, rows, waves[wave]);
       __builtin_amdgcn_sched_barrier(0);
     };
-    for (int s0 = k_lo, s1; s0 < k_hi; s0 = s1) {
-      s1 = k_hi;
-      if constexpr (!UNIFORM) {
-        // As many whole units as the entries that fit in LDS reach.
+    if (!WHOLE) __syncthreads();  // (the sweep before's results are read)
+    // This wave's first block from s0: also where it has none before s1 (the last key's rows then),
+    // so that what waits for q below waits for no more.
+    auto begin = [&](int key0) {
+      next = B::look(p, keys, key0);
+      rows = x.load_k(p, keys, waves[wave], next, key0);
+      x.load_v(p, rows, waves[wave]);
+      next = B::look(p, keys, key0 + kStep);
+    };
+    auto go_on = [&](int key0, int s1) {
+      if (key0 >= s1) return;
+      for (; key0 + kStep < s1; key0 += kStep) fold(key0, std::true_type{});
+      fold(key0, std::false_type{});
+    };
+    if constexpr (UNIFORM) {
+      if (k_lo < k_hi) {
+        begin(k_lo + kBlock * wave);
+        lay_q();
+        __syncthreads();
+        go_on(k_lo + kBlock * wave, k_hi);
+      }
+    } else {
+      lay_q();
+      for (int s0 = k_lo, s1; s0 < k_hi; s0 = s1) {
+        // As many whole steps as the entries that fit in LDS reach.
         keys.first = thd::quotient(s0, p.pages.by_page);
         s1 = (int)min((int64_t)k_hi, s0 + ((int64_t)(keys.first + kEntries) * p.pages.page - s0) / kStep * kStep);
         keys.last = min(last, s1 - 1);
         const int n = thd::quotient(s1 - 1, p.pages.by_page) - keys.first + 1;
-        __syncthreads();  // (what was there is read)
+        if (s0 > k_lo) __syncthreads();  // (what was there is read)
         for (int i = threadIdx.x; i < n; i += 64 * NW) entries[i] = keys.table[keys.first + i];
         __syncthreads();
-      }
-      int key0 = s0 + kBlock * wave;
-      if (key0 < s1) {
-        rows = x.load_k(p, keys, waves[wave], key0);
-        x.load_v(p, rows, waves[wave]);
-      }
-      if constexpr (UNIFORM) __syncthreads();  // (q is there)
-      if (key0 < s1) {
-        for (; key0 + kStep < s1; key0 += kStep) fold(key0, std::true_type{});
-        fold(key0, std::false_type{});
+        begin(s0 + kBlock * wave);
+        go_on(s0 + kBlock * wave, s1);
       }
     }
     l += __shfl_xor(l, 16, 64);
@@ -700,9 +755,9 @@ __global__ __launch_bounds__(1024) void paged_attn_join(PagedArgs p) {
   __shared__ f32x4 Os[1024];
   const int h = blockIdx.x, pos = blockIdx.y, b = blockIdx.z;
   const int hk = thd::quotient(h, p.by_group), row = pos * p.group + h - hk * p.group, tile = row / kRows;
-  const int32_t* pieces = p.pieces + 2 * ((int64_t)b * p.sweeps + hk * p.tiles + tile);
+  const constant_i32 pieces = (constant_i32)p.pieces + 2 * ((int64_t)b * p.sweeps + hk * p.tiles + tile);
   const int at0 = pieces[0], n = pieces[1];
-  const Sequence seq = sequence_of(p, b);
+  const Sequence seq = sequence_of_all(p, b);
   if (pos >= seq.count) return;
   const int quad = threadIdx.x % quads, mine = threadIdx.x / quads, groups = blockDim.x / quads;
   float m = -INFINITY, l = 0.0f;
