@@ -745,21 +745,22 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
   }
 }
 
-// The rows whose sweep lies in several pieces, or has no keys: a workgroup a row, its
-// threads in groups of D / 4, each of which takes every so manieth piece, four
-// loads at a time; then the groups' results in order.
+// The rows whose sweep lies in several pieces, or has no keys: a workgroup for 64
+// features of a row, its threads in groups of 16, each of which takes every so
+// manieth piece, four loads at a time; then the groups' results in order.
 template <int D, bool F16>
 __global__ __launch_bounds__(1024) void paged_attn_join(PagedArgs p) {
-  constexpr int quads = D / 4;
-  __shared__ float Ms[1024 / quads], Ls[1024 / quads];
+  constexpr int slices = D / 64;
+  __shared__ float Ms[64], Ls[64];
   __shared__ f32x4 Os[1024];
-  const int h = blockIdx.x, pos = blockIdx.y, b = blockIdx.z;
+  const int h = blockIdx.x / slices, pos = blockIdx.y, b = blockIdx.z;
   const int hk = thd::quotient(h, p.by_group), row = pos * p.group + h - hk * p.group, tile = row / kRows;
   const constant_i32 pieces = (constant_i32)p.pieces + 2 * ((int64_t)b * p.sweeps + hk * p.tiles + tile);
   const int at0 = pieces[0], n = pieces[1];
   const Sequence seq = sequence_of_all(p, b);
   if (pos >= seq.count) return;
-  const int quad = threadIdx.x % quads, mine = threadIdx.x / quads, groups = blockDim.x / quads;
+  const int quad = threadIdx.x % 16, mine = threadIdx.x / 16, groups = blockDim.x / 16;
+  const int f = 64 * (blockIdx.x % slices) + 4 * quad;
   float m = -INFINITY, l = 0.0f;
   f32x4 acc = {};
   if (seq.blocks > 0) {
@@ -773,7 +774,7 @@ __global__ __launch_bounds__(1024) void paged_attn_join(PagedArgs p) {
         // The first in either of its workgroup's places, the others in their first.
         const int64_t from = (int64_t)(piece ? (at0 & ~1) + 2 * piece : at0) * kRows + row % kRows;
         x[i] = reinterpret_cast<const f32x2*>(p.part_ml)[from];
-        y[i] = *reinterpret_cast<const f32x4*>(p.part + from * D + 4 * quad);
+        y[i] = *reinterpret_cast<const f32x4*>(p.part + from * D + f);
       }
       float mn = m;
 #pragma unroll
@@ -803,17 +804,17 @@ __global__ __launch_bounds__(1024) void paged_attn_join(PagedArgs p) {
       for (int i = 0; i < groups; ++i) {
         const float a = __builtin_amdgcn_exp2f(Ms[i] - shift);
         l += a * Ls[i];
-        acc += a * Os[i * quads + quad];
+        acc += a * Os[i * 16 + quad];
       }
       m = mn;
     }
   }
   if (mine > 0) return;
   const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
-  if (4 * quad < p.head_dim)
-    *reinterpret_cast<u32x2_any*>(p.o + b * p.q_sb + h * p.q_sh + pos * p.q_ss + 4 * quad) =
+  if (f < p.head_dim)
+    *reinterpret_cast<u32x2_any*>(p.o + b * p.q_sb + h * p.q_sh + pos * p.q_ss + f) =
         u32x2{rounded2<F16>(acc[0] * inv, acc[1] * inv), rounded2<F16>(acc[2] * inv, acc[3] * inv)};
-  if (quad == 0 && p.lse) p.lse[((int64_t)b * p.seq + pos) * p.heads + h] = (m + log2f(l)) * kLn2;
+  if (f == 0 && p.lse) p.lse[((int64_t)b * p.seq + pos) * p.heads + h] = (m + log2f(l)) * kLn2;
 }
 
 // Whether each sweep is one workgroup's.
@@ -857,8 +858,9 @@ int launch(const th_paged_desc* d, th_launch** out) {
   if (!WHOLE) {
     // Threads for about as many pieces as a sweep has at the most.
     int threads = 256;
-    while (threads < 1024 && threads / (D / 4) * 4 < a.workers / sweeps) threads *= 2;
-    end = b.kernel((const void*)paged_attn_join<D, F16>, "paged_attn_join", dim3(d->heads, d->seq, d->batch), dim3(threads), 0, a);
+    while (threads < 1024 && threads / 16 * 4 < a.workers / sweeps) threads *= 2;
+    end = b.kernel((const void*)paged_attn_join<D, F16>, "paged_attn_join", dim3(d->heads * (D / 64), d->seq, d->batch),
+                   dim3(threads), 0, a);
     const uint64_t at_o = b.workspace((uint64_t)a.workers * 2 * kRows * D * sizeof(float));
     const uint64_t at_ml = b.workspace((uint64_t)a.workers * 2 * kRows * 2 * sizeof(float));
     const uint64_t at_pieces = b.workspace((uint64_t)sweeps * 2 * sizeof(int32_t));
