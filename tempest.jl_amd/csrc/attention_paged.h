@@ -906,9 +906,10 @@ int launch(const th_paged_desc* d, th_launch** out) {
 template <int D>
 int launch_dim(const th_paged_desc* d, th_launch** out) {
   if (d->cache.head_dim != D) return launch<D, false, false, false>(d, out);
-  if (d->cache.page % 16 != 0 || d->cache.strides[1] >= (1 << 26)) return launch<D, true, false, false>(d, out);
-  return d->seq > 1 || d->heads / d->cache.heads > kRows ? launch<D, true, true, false>(d, out)
-                                                         : launch<D, true, true, true>(d, out);
+  const bool uniform = d->cache.page % 16 == 0 && d->cache.strides[1] < (1 << 26);
+  if (d->seq > 1 || d->heads / d->cache.heads > kRows)
+    return uniform ? launch<D, true, true, false>(d, out) : launch<D, true, false, false>(d, out);
+  return uniform ? launch<D, true, true, true>(d, out) : launch<D, true, false, true>(d, out);
 }
 
 }  // namespace
