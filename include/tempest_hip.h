@@ -786,10 +786,10 @@ int th_build_rotary(const th_rotary_desc* desc, th_launch** host_out);
 /* K and V arrays (features, heads, positions in a page, pages), bf16, fp16 or
  * e4m3, at strides along heads, positions and pages (elements, features
  * adjacent; one stride set for both, heads and positions in either order).
- * head_dim is a multiple of 8 up to 256, the arrays 16-byte aligned, strides
+ * head_dim is a multiple of 8 up to 256, the arrays 16-byte aligned (scales 4-byte), strides
  * multiples of 8.
  * TH_E4M3: a byte a feature, and for each 32 features of a row one byte e, the scale
- * 2^(e - 127): what is held is the code's value times the scale.  The scale of
+ * 2^(e - 127), e from 1 to 254: what is held is the code's value times the scale.  The scale of
  * the feature at element x of k is k_scales[x / 32], so head_dim and the strides are
  * multiples of 32.
  * A sequence's position p is in page table[p / page, b] at place p % page:
@@ -797,7 +797,7 @@ int th_build_rotary(const th_rotary_desc* desc, th_launch** host_out);
  * table_pages * b.  An entry outside 0..pages-1 names no page: nothing is
  * written there, what is read there is zero, and no query sees a key there.
  * lengths, int32 (batch), is how many positions each sequence holds, new ones
- * included (taken into 0..table_pages * page); counts, int32 (batch) or NULL, how
+ * included (taken into 0..table_pages * page, at most 2^30); counts, int32 (batch) or NULL, how
  * many of the seq new ones are real (into 0..seq; NULL: all seq): the j-th new
  * position of sequence b is lengths[b] - counts[b] + j.  The device holds table,
  * lengths and counts and reads them when the launch runs.

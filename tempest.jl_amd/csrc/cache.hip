@@ -170,6 +170,8 @@ int build(const th_cache_desc* d, bool write, th_launch** out) {
   TH_REQUIRE(reinterpret_cast<uintptr_t>(d->k) % 2 == 0 && reinterpret_cast<uintptr_t>(d->v) % 2 == 0,
              std::string(what) + ": k and v must be aligned to their elements");
   TH_REQUIRE(d->table && d->lengths, std::string(what) + ": null table or lengths");
+  TH_REQUIRE(th::aligned4(d->table) && th::aligned4(d->lengths) && th::aligned4(d->counts),
+             std::string(what) + ": table, lengths and counts must be 4-byte aligned");
   TH_REQUIRE(write || !d->counts, "cache read: counts are for writing");
   const int64_t extents[3] = {c.heads, d->seq, d->batch};
   for (int64_t s : d->strides) TH_REQUIRE(s >= 0, std::string(what) + ": strides must not be negative");
@@ -247,12 +249,14 @@ int check_cache(const th_cache& c, int32_t dtype, int32_t table_pages, const cha
   TH_REQUIRE(c.heads > 0 && c.heads <= 65535, w + ": the cache's heads must be 1..65535");
   TH_REQUIRE(c.page > 0 && c.pages > 0 && (int64_t)c.page * c.pages <= 0x7fffffff,
              w + ": page and pages must be positive, and their product under 2^31");
-  TH_REQUIRE(table_pages > 0 && (int64_t)table_pages * c.page <= 0x7fffffff,
-             w + ": table_pages must be positive, and table_pages * page under 2^31");
+  TH_REQUIRE(table_pages > 0 && (int64_t)table_pages * c.page <= (1 << 30),
+             w + ": table_pages must be positive, and table_pages * page at most 2^30");
   TH_REQUIRE(c.k && c.v, w + ": null cache");
   TH_REQUIRE(reinterpret_cast<uintptr_t>(c.k) % 16 == 0 && reinterpret_cast<uintptr_t>(c.v) % 16 == 0,
              w + ": the cache's arrays must be 16-byte aligned");
   TH_REQUIRE(c.dtype != TH_E4M3 || (c.k_scales && c.v_scales), w + ": an e4m3 cache needs k_scales and v_scales");
+  TH_REQUIRE(reinterpret_cast<uintptr_t>(c.k_scales) % 4 == 0 && reinterpret_cast<uintptr_t>(c.v_scales) % 4 == 0,
+             w + ": the scales must be 4-byte aligned");
   for (int64_t s : c.strides)
     TH_REQUIRE(s >= 0 && s % unit == 0, w + ": the cache's strides must be multiples of 8 (of 32 for e4m3)");
   const int64_t extents[3] = {c.heads, c.page, c.pages};

@@ -222,6 +222,7 @@ int build(const th_rotary_desc* d, th_launch** out) {
   TH_REQUIRE((d->flags & ~(TH_ROTARY_PAIRS | TH_ROTARY_INVERSE)) == 0, "rotary: unknown flags");
   TH_REQUIRE((int64_t)d->heads + d->kv_heads <= 65535, "rotary: heads and kv_heads must be at most 65535 together");
   TH_REQUIRE(d->positions && d->freqs, "rotary: null positions or freqs");
+  TH_REQUIRE(th::aligned4(d->positions) && th::aligned4(d->freqs), "rotary: positions and freqs must be 4-byte aligned");
   const int half = d->rotary_dim / 2, size = d->dtype == TH_F32 ? 4 : 2;
   RotaryArgs a{};
   int sum = 0;

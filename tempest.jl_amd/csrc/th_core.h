@@ -258,6 +258,7 @@ inline Divisor divisor(int32_t d) {
   return {(uint32_t)((uint64_t(1) << (31 + l)) / (uint32_t)d + 1), (uint32_t)(31 + l)};
 }
 
+inline bool aligned4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 // Rows of `row` elements at these strides lie apart: ordered by stride, each
 // stride passes what the shorter ones span (cache.hip).  Extents of 1 need none.
 bool rows_apart(int64_t row, const int64_t* strides, const int64_t* extents, int n);

@@ -100,7 +100,20 @@ CASES = [  # B, S, H, KV, D, page, cap, dtype, e4m3, outer, lengths, counts, mas
     (2, 1, 2, 2, 64, 16, 300, "bf16", False, False, [4000, -5], None, {}),
     (2, 1, 4, 2, 64, 16, 9000, "bf16", False, False, [9000, 1500], None, {"window": 1}),
     (40, 1, 8, 2, 128, 16, 700, "bf16", False, False, [(37 * i) % 701 for i in range(40)], None, {}),
-    (1, 1, 8, 8, 64, 64, 9000, "bf16", True, False, [8999], None, {"scale": 0.3})]
+    (1, 1, 8, 8, 64, 64, 9000, "bf16", True, False, [8999], None, {"scale": 0.3}),
+    # Long tables: the keys divided among workgroups, pieces joined.
+    (150, 1, 4, 1, 64, 64, 1600, "bf16", False, False, [(211 * i) % 1601 if i % 3 else 0 for i in range(150)], None, {}),
+    (70, 2, 2, 1, 64, 7, 1500, "f16", True, False, [(97 * i) % 1501 for i in range(70)], [i % 3 for i in range(70)], {}),
+    (3, 1, 16, 2, 256, 16, 1200, "f16", False, True, [1200, 0, 33], None, {}),
+    (2, 3, 6, 2, 256, 32, 1000, "bf16", True, False, [1000, 999], [3, 2], {}),
+    (2, 1, 4, 2, 224, 16, 1000, "bf16", True, True, [1000, 515], None, {}),
+    (2, 4, 4, 2, 80, 5, 2500, "f16", False, False, [2500, 1], [4, 3], {"window": 1900}),
+    (1, 1, 40, 2, 128, 128, 2000, "bf16", False, False, [1999], None, {}),
+    (2, 20, 4, 1, 128, 16, 1500, "bf16", False, False, [1500, 37], [20, 11], {}),
+    (2, 3, 4, 2, 128, 24, 1500, "bf16", True, False, [1411, 1500], None, {"causal": False}),
+    (1, 1, 2, 1, 64, 1, 5000, "bf16", False, False, [4997], None, {}),
+    (1, 2, 8, 2, 128, 1, 2900, "f16", True, True, [2900], None, {}),
+    (1, 1, 1, 1, 128, 16, 40000, "bf16", True, False, [40000], None, {})]
 
 
 @pytest.mark.parametrize("B,S,H,KV,D,page,cap,dtype,e4m3,outer,lengths,counts,masks", CASES)
@@ -123,18 +136,19 @@ def test_paged(target, B, S, H, KV, D, page, cap, dtype, e4m3, outer, lengths, c
 
 
 @pytest.mark.parametrize("dtype,e4m3", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
-@pytest.mark.parametrize("S,window", [(1, 0), (4, 0), (4, 40), (9, 3)])
-def test_what_no_query_sees_may_be_anything(target, dtype, e4m3, S, window):
+@pytest.mark.parametrize("S,window,page,cap", [(1, 0, 8, 200), (4, 0, 8, 200), (4, 40, 8, 200), (9, 3, 8, 200), (1, 0, 16, 1600),
+                                               (3, 0, 16, 1600), (3, 1500, 8, 1600), (4, 0, 16, 200)])
+def test_what_no_query_sees_may_be_anything(target, dtype, e4m3, S, window, page, cap):
     """NaN and infinities behind the lengths, before the window, in the new
     rows of later positions and in pages no entry names (for the query that does not see them)."""
-    announce("paged unseen", dtype, e4m3, S, window)
-    B, H, KV, D, page, cap = 2, 4, 2, 64, 8, 200
+    announce("paged unseen", dtype, e4m3, S, window, page, cap)
+    B, H, KV, D = 2, 4, 2, 64
     c = Paged(B, cap, KV, D, page, dtype, e4m3)
     gen = torch.Generator(device="cuda").manual_seed(S + window)
     _fill(c, gen, cap)
     q = rows(gen, dtype, B, S, H, D, spread=False)
-    n = ints(150, 97)
-    lengths = [150, 97]
+    lengths = [150, 97] if cap == 200 else [1550, 1497]
+    n = ints(*lengths)
 
     def run():
         o, lse = torch.full_like(q, 6.0), torch.full((B, S, H), 6.0, device="cuda")
@@ -180,11 +194,12 @@ def test_what_no_query_sees_may_be_anything(target, dtype, e4m3, S, window):
         c.k[where] = keep[0]
 
 
-@pytest.mark.parametrize("dtype,e4m3", [("bf16", False), ("f16", True)])
-def test_entries_that_name_no_page(target, dtype, e4m3):
+@pytest.mark.parametrize("dtype,e4m3,page,cap,S", [("bf16", False, 8, 200, 2), ("f16", True, 8, 200, 2), ("bf16", True, 16, 2000, 1),
+                                                    ("bf16", False, 16, 304, 1), ("f16", False, 7, 2100, 3)])
+def test_entries_that_name_no_page(target, dtype, e4m3, page, cap, S):
     """No query sees a key there: holes in a sequence, one that has no page at all."""
-    announce("paged bad pages", dtype, e4m3)
-    B, S, H, KV, D, page, cap = 3, 2, 4, 2, 64, 8, 200
+    announce("paged bad pages", dtype, e4m3, page, cap, S)
+    B, H, KV, D = 3, 4, 2, 64
     c = Paged(B, cap, KV, D, page, dtype, e4m3)
     gen = torch.Generator(device="cuda").manual_seed(3)
     _fill(c, gen, cap)
@@ -300,7 +315,7 @@ def test_recorded_and_shared_workspaces(target):
     the lengths the device then holds, beside eager runs; every result its own eager one."""
     announce("paged graphs")
     cases = []
-    for i, (D, e4m3, cap) in enumerate([(64, False, 3000), (128, True, 5000)]):
+    for i, (D, e4m3, cap) in enumerate([(64, False, 3000), (128, True, 5000), (256, False, 3000)]):
         c = Paged(2, cap, 2, D, 16, "bf16", e4m3)
         gen = torch.Generator(device="cuda").manual_seed(i)
         _fill(c, gen, cap)

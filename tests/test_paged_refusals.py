@@ -53,7 +53,7 @@ def _attend(cache=None, **over):
 
 BAD_CACHES = [dict(dtype=L.F32), dict(head_dim=60), dict(head_dim=264), dict(head_dim=0), dict(heads=0), dict(page=0),
               dict(pages=0), dict(page=1 << 16, pages=1 << 15), dict(k=0), dict(v=P + 8), dict(dtype=L.E4M3),
-              dict(dtype=L.E4M3, k_scales=P, v_scales=P, head_dim=80), dict(strides=(64, 100, 2048)),
+              dict(dtype=L.E4M3, k_scales=P, v_scales=P, head_dim=80), dict(dtype=L.E4M3, k_scales=P, v_scales=P + 2), dict(strides=(64, 100, 2048)),
               dict(strides=(64, -128, 2048)), dict(strides=(64, 64, 2048)), dict(strides=(64, 128, 1024)),
               dict(**E4M3, strides=(80, 160, 2560))]
 
@@ -75,7 +75,8 @@ def test_a_cache_every_kernel_takes(f, good):
 @pytest.mark.parametrize("f,bad", [
     (_write, dict(batch=0)), (_write, dict(batch=65536)), (_write, dict(seq=0)), (_write, dict(k=0)),
     (_write, dict(v=P + 1)), (_write, dict(table=0)), (_write, dict(lengths=0)), (_write, dict(table_pages=0)),
-    (_write, dict(table_pages=1 << 27)), (_write, dict(strides=(-64, 128, 384))), (_write, dict(seq=1 << 28)),
+    (_write, dict(table_pages=1 << 27)), (_write, dict(counts=P + 2)), (_read, dict(table=P + 1)),
+    (_attend, dict(lengths=P + 2)), (_attend, dict(lse=P + 2)), (_write, dict(strides=(-64, 128, 384))), (_write, dict(seq=1 << 28)),
     (_read, dict(strides=(64, 128, 256))), (_read, dict(strides=(32, 128, 384))), (_read, dict(k=0)),
     (_attend, dict(heads=3)), (_attend, dict(heads=0)), (_attend, dict(window=-1)),
     (_attend, dict(window=5, causal=False)), (_attend, dict(q=0)), (_attend, dict(o=P + 1)),
@@ -118,7 +119,7 @@ def _rotary(**over):
 @pytest.mark.parametrize("bad", [
     dict(dtype=L.E4M3), dict(batch=0), dict(seq=0), dict(heads=0), dict(kv_heads=-1), dict(head_dim=0),
     dict(head_dim=2048), dict(rotary_dim=33), dict(rotary_dim=66), dict(sections=[]), dict(sections=[16, 8]),
-    dict(sections=[40, -8]), dict(sections=[32, 1]), dict(positions=0), dict(freqs=0), dict(q=0), dict(k_out=0),
+    dict(sections=[40, -8]), dict(sections=[32, 1]), dict(positions=0), dict(freqs=0), dict(positions=P + 2), dict(q=0), dict(k_out=0),
     dict(q=P + 1), dict(dtype=L.F32, k=P + 2), dict(position_strides=(1, 1, -5)), dict(q_strides=(64, 256, -1)),
     dict(q_out_strides=(32, 256, 1280)), dict(k_out_strides=(64, 0, 640)),
     dict(q_out=P, q_strides=(64, 256, 1280), q_out_strides=(64, 512, 2560)), dict(batch=1 << 20, seq=1 << 20),
