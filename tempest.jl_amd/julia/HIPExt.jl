@@ -917,6 +917,130 @@ function build(::HIPDeltaNet, t::HIPTarget, b::Binding, resources)
     (l, "chunked gated DeltaNet" * (grad ? " gradient" : "") * ": " * describe(l))
 end
 
+# ---- rotary positions, a key-value cache in pages -------------------------------------------
+#
+# No program of Tempest's spells these as one group (a rotary turn is a pointwise
+# group of its own, a page a gathered read, a cache's write a fold by key that
+# writes), so no template claims them: a host that serves a model builds their launches
+# and runs them beside a compiled program's, or records them with it.  Arrays are
+# (features, heads, positions, batch) device arrays whose features are adjacent.
+
+struct RotaryDesc
+    dtype::Int32; batch::Int32; seq::Int32; heads::Int32; kv_heads::Int32; head_dim::Int32; rotary_dim::Int32
+    axes::Int32; sections::NTuple{4, Int32}; flags::Int32; reserved::Int32
+    q::Ptr{Cvoid}; k::Ptr{Cvoid}; q_out::Ptr{Cvoid}; k_out::Ptr{Cvoid}
+    q_strides::NTuple{3, Int64}; k_strides::NTuple{3, Int64}
+    q_out_strides::NTuple{3, Int64}; k_out_strides::NTuple{3, Int64}
+    positions::Ptr{Cvoid}; freqs::Ptr{Cvoid}; position_strides::NTuple{3, Int64}
+end
+
+struct CCache
+    dtype::Int32; heads::Int32; head_dim::Int32; page::Int32; pages::Int32; reserved::Int32
+    k::Ptr{Cvoid}; v::Ptr{Cvoid}; k_scales::Ptr{UInt8}; v_scales::Ptr{UInt8}
+    strides::NTuple{3, Int64}
+end
+
+struct CacheDesc
+    cache::CCache; dtype::Int32; batch::Int32; seq::Int32; table_pages::Int32
+    k::Ptr{Cvoid}; v::Ptr{Cvoid}; strides::NTuple{3, Int64}
+    table::Ptr{Int32}; lengths::Ptr{Int32}; counts::Ptr{Int32}
+end
+
+struct PagedDesc
+    cache::CCache; dtype::Int32; batch::Int32; heads::Int32; seq::Int32; table_pages::Int32
+    causal::Int32; window::Int32; scale::Float32
+    q::Ptr{Cvoid}; o::Ptr{Cvoid}; lse::Ptr{Cvoid}; q_strides::NTuple{3, Int64}
+    table::Ptr{Int32}; lengths::Ptr{Int32}; counts::Ptr{Int32}
+end
+
+paged_dtype(::Type{Float32}) = Int32(0)
+paged_dtype(::Type{Float16}) = Int32(4)
+paged_dtype(T::Type) = T === Tempest.BFloat16 ? Int32(1) : throw(ArgumentError("no device array of $T here"))
+
+# The address of a device array, or null for `nothing`.
+buffer_address(x) = x === nothing ? C_NULL : Ptr{Cvoid}(device_address(x))
+# An array's strides along its axes 2, 3 and 4.
+row_strides(x) = (Int64(stride(x, 2)), Int64(stride(x, 3)), Int64(stride(x, 4)))
+
+"""
+    rotary(t, q, k, q_out, k_out, positions, freqs; sections, pairs = false, inverse = false)
+
+The launch that turns `q` and `k` (`nothing`: `q` alone) by `positions` (Int32, (axes, positions,
+batch)) into `q_out` and `k_out`, which may be `q` and `k`: pair `p` by the position on its axis times
+`freqs[p]` (Float32), the first `sections[1]` pairs on axis 1 and so on.  `inverse` turns back, the
+gradient.
+"""
+function rotary(t::HIPTarget, q, k, q_out, k_out, positions, freqs; sections = (length(freqs),), pairs = false,
+                inverse = false)
+    kk, ko = k === nothing ? (q, q_out) : (k, k_out)
+    d = Ref(RotaryDesc(paged_dtype(eltype(q)), size(q, 4), size(q, 3), size(q, 2), k === nothing ? 0 : size(k, 2),
+        size(q, 1), 2length(freqs), length(sections), ntuple(i -> Int32(get(sections, i, 0)), 4),
+        (pairs ? 1 : 0) | (inverse ? 2 : 0), 0, buffer_address(q), buffer_address(k), buffer_address(q_out), buffer_address(k_out),
+        row_strides(q), row_strides(kk), row_strides(q_out), row_strides(ko), buffer_address(positions), buffer_address(freqs),
+        (Int64(stride(positions, 1)), Int64(stride(positions, 2)), Int64(stride(positions, 3)))))
+    out = Ref{Ptr{Cvoid}}()
+    check(ccall((:th_build_rotary, LIB), Cint, (Ptr{RotaryDesc}, Ptr{Ptr{Cvoid}}), d, out), "th_build_rotary")
+    HIPLaunch(out[], Any[q, k, q_out, k_out, positions, freqs], Tuple{Int, Int, Int, DataType}[], t.pool)
+end
+
+"""
+    PagedCache(k, v; k_scales = nothing, v_scales = nothing)
+
+A cache's device arrays, (features, heads, positions in a page, pages): Float16 or BFloat16, or UInt8
+codes of e4m3 with their scale bytes, (features / 32, heads, positions in a page, pages).
+"""
+struct PagedCache
+    k::Any
+    v::Any
+    k_scales::Any
+    v_scales::Any
+    PagedCache(k, v; k_scales = nothing, v_scales = nothing) = new(k, v, k_scales, v_scales)
+end
+paged_dtype(c::PagedCache) = eltype(c.k) === UInt8 ? Int32(5) : paged_dtype(eltype(c.k))
+ccache(c::PagedCache) = CCache(paged_dtype(c), size(c.k, 2), size(c.k, 1), size(c.k, 3), size(c.k, 4), 0,
+    buffer_address(c.k), buffer_address(c.v), buffer_address(c.k_scales), buffer_address(c.v_scales), row_strides(c.k))
+paged_values(c::PagedCache) = Any[c.k, c.v, c.k_scales, c.v_scales]
+
+cache_desc(c::PagedCache, k, v, table, lengths, counts) = Ref(CacheDesc(ccache(c), paged_dtype(eltype(k)), size(k, 4),
+    size(k, 3), size(table, 1), buffer_address(k), buffer_address(v), row_strides(k), buffer_address(table), buffer_address(lengths),
+    buffer_address(counts)))
+
+"""
+    cache_write(t, cache, k, v, table, lengths; counts = nothing)
+    cache_read(t, cache, k, v, table, lengths)
+
+The launches that write the new rows `k` and `v` at the ends of the sequences, and that read the
+sequences back: `table` (Int32, (pages of a sequence, batch)), `lengths` and `counts` (Int32, batch).
+"""
+function cache_write(t::HIPTarget, cache::PagedCache, k, v, table, lengths; counts = nothing)
+    d, out = cache_desc(cache, k, v, table, lengths, counts), Ref{Ptr{Cvoid}}()
+    check(ccall((:th_build_cache_write, LIB), Cint, (Ptr{CacheDesc}, Ptr{Ptr{Cvoid}}), d, out), "th_build_cache_write")
+    HIPLaunch(out[], [paged_values(cache); Any[k, v, table, lengths, counts]], Tuple{Int, Int, Int, DataType}[], t.pool)
+end
+function cache_read(t::HIPTarget, cache::PagedCache, k, v, table, lengths)
+    d, out = cache_desc(cache, k, v, table, lengths, nothing), Ref{Ptr{Cvoid}}()
+    check(ccall((:th_build_cache_read, LIB), Cint, (Ptr{CacheDesc}, Ptr{Ptr{Cvoid}}), d, out), "th_build_cache_read")
+    HIPLaunch(out[], [paged_values(cache); Any[k, v, table, lengths]], Tuple{Int, Int, Int, DataType}[], t.pool)
+end
+
+"""
+    paged_attention(t, cache, q, o, table, lengths; lse = nothing, counts = nothing, causal = true, window = 0, scale = 0)
+
+The launch of attention of the sequences' last positions `q` over the cache, into `o` (laid out as `q`).
+"""
+function paged_attention(t::HIPTarget, cache::PagedCache, q, o, table, lengths; lse = nothing, counts = nothing,
+                         causal = true, window = 0, scale = 0)
+    row_strides(o) == row_strides(q) || throw(ArgumentError("o must be laid out as q"))
+    d = Ref(PagedDesc(ccache(cache), paged_dtype(eltype(q)), size(q, 4), size(q, 2), size(q, 3), size(table, 1),
+        causal, window, scale, buffer_address(q), buffer_address(o), buffer_address(lse), row_strides(q), buffer_address(table), buffer_address(lengths),
+        buffer_address(counts)))
+    out = Ref{Ptr{Cvoid}}()
+    check(ccall((:th_build_attention_paged, LIB), Cint, (Ptr{PagedDesc}, Ptr{Ptr{Cvoid}}), d, out),
+          "th_build_attention_paged")
+    HIPLaunch(out[], [paged_values(cache); Any[q, o, lse, table, lengths, counts]], Tuple{Int, Int, Int, DataType}[],
+        t.pool)
+end
+
 # ---- the floor: any group, generated -----------------------------------------------------
 #
 # The reference's floor turns a group into Julia code (scalar_kernel,
