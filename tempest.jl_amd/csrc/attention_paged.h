@@ -379,7 +379,7 @@ __device__ __forceinline__ void split2_f16(float a, float b, uint32_t& w0, uint3
 
 // Waves a SIMD that the registers are kept to.
 constexpr int waves_of(int D, bool SINGLE, bool WHOLE) {
-  if (WHOLE) return D > 64 ? 2 : 4;
+  if (WHOLE) return D > 64 || !SINGLE ? 2 : 4;
   return D > 128 ? 1 : D > 64 ? (SINGLE ? 3 : 2) : SINGLE ? 4 : 3;
 }
 
@@ -907,7 +907,10 @@ int launch(const th_paged_desc* d, th_launch** out) {
 }
 template <int D, bool EXACT, bool UNIFORM, bool SINGLE>
 int launch(const th_paged_desc* d, th_launch** out) {
-  return whole_sweeps(d) ? launch<D, EXACT, UNIFORM, SINGLE, true>(d, out) : launch<D, EXACT, UNIFORM, SINGLE, false>(d, out);
+  // Whole sweeps of several positions of 256 features lack registers, the more with the
+  // scalar addresses (12.5 us and 9.3 without, 2 x 64 positions of 8 heads in bf16).
+  constexpr bool scalar = UNIFORM && (SINGLE || D < 256);
+  return whole_sweeps(d) ? launch<D, EXACT, scalar, SINGLE, true>(d, out) : launch<D, EXACT, UNIFORM, SINGLE, false>(d, out);
 }
 // Pages in sixteens (and rows of a half block within 31 bits) take the scalar addresses.
 template <int D>
