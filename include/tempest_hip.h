@@ -855,7 +855,7 @@ int th_build_cache_read(const th_cache_desc* desc, th_launch** host_out);
  * counts[b] of o and lse stay.  What a key or value holds that no query sees may be
  * anything, NaN included.
  * q and o are (d, heads, positions, batch) at q_strides, bf16 or fp16, the cache's
- * type or beside TH_E4M3; any alignment.  lse (if non-NULL) as th_build_attention_fwd
+ * type or beside TH_E4M3; any alignment; o may be q.  lse (if non-NULL) as th_build_attention_fwd
  * writes it; heads a multiple of the cache's heads; scale <= 0 means
  * 1/sqrt(head_dim).  The weights are fp32's, as are all sums.  The keys are read once for
  * every 16 rows (seq * heads / cache heads).  Workspace: the split's partial results.

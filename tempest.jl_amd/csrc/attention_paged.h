@@ -848,7 +848,8 @@ int launch(const th_paged_desc* d, th_launch** out) {
   a.pages = th::pages_of(cache, d->table_pages, d->table, d->lengths, d->counts);
   a.q_sh = d->q_strides[0], a.q_ss = d->q_strides[1], a.q_sb = d->q_strides[2];
   a.seq = d->seq, a.heads = d->heads, a.kv_heads = cache.heads, a.batch = d->batch, a.head_dim = cache.head_dim;
-  a.causal = d->causal != 0, a.window = d->window;
+  a.causal = d->causal != 0;
+  a.window = std::min(d->window, 1 << 30);  // (a table's most positions: a wider one would pass 32 bits below position 0)
   a.scale = d->scale > 0 ? d->scale : 1.0f / sqrtf((float)cache.head_dim);
   a.group = d->heads / cache.heads;
   a.tiles = (int)(((int64_t)d->seq * a.group + kRows - 1) / kRows);

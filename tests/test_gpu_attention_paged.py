@@ -135,6 +135,40 @@ def test_paged(target, B, S, H, KV, D, page, cap, dtype, e4m3, outer, lengths, c
     assert torch.equal(o, o2)
 
 
+@pytest.mark.parametrize("page,cap", [(16, 200), (7, 200), (16, 2000), (7, 2000)])
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31 - 1])
+def test_the_widest_windows(target, page, cap, window):
+    """More new positions than a sequence holds, some of them below position 0: no
+    window reaches past 32 bits there."""
+    announce("paged widest window", page, cap, window)
+    B, S, H, KV, D = 4, 9, 4, 2, 64
+    c = Paged(B, cap, KV, D, page, "bf16", False)
+    gen = torch.Generator(device="cuda").manual_seed(cap)
+    _fill(c, gen, cap)
+    q = rows(gen, "bf16", B, S, H, D, spread=False)
+    n, m = ints(0, 3, cap, 1), ints(9, 7, 9, 5)
+    o, lse = torch.full_like(q, 6.0), torch.full((B, S, H), 6.0, device="cuda")
+    _attend(c, q, o, lse, n, m, window=window)()
+    torch.cuda.synchronize()
+    _check(c, q, o, lse, n, m, was=6.0, window=window)
+
+
+@pytest.mark.parametrize("S,page,cap,e4m3", [(1, 16, 200, False), (5, 7, 200, True), (1, 7, 6000, True), (9, 16, 3000, False)])
+def test_over_its_queries(target, S, page, cap, e4m3):
+    announce("paged in place", S, page, cap, e4m3)
+    B, H, KV, D = 3, 8, 2, 128
+    c = Paged(B, cap, KV, D, page, "bf16", e4m3)
+    gen = torch.Generator(device="cuda").manual_seed(cap)
+    _fill(c, gen, cap)
+    q = rows(gen, "bf16", B, S, H, D, spread=False)
+    n, m = ints(cap, 0, cap // 2), ints(S, S, S - 1)
+    o, lse = q.clone(), torch.empty((B, S, H), device="cuda")
+    _attend(c, q, o, lse, n, m)()
+    _attend(c, q, q, lse, n, m)()
+    torch.cuda.synchronize()
+    assert torch.equal(o, q)
+
+
 @pytest.mark.parametrize("dtype,e4m3", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
 @pytest.mark.parametrize("S,window,page,cap", [(1, 0, 8, 200), (4, 0, 8, 200), (4, 40, 8, 200), (9, 3, 8, 200), (1, 0, 16, 1600),
                                                (3, 0, 16, 1600), (3, 1500, 8, 1600), (4, 0, 16, 200)])
