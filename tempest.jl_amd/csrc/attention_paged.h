@@ -4,18 +4,27 @@
 //
 // The work is the cache's bytes: each (sequence, cache head) reads its K and V
 // once for the 16 query rows (position, head of the group) that are the columns of one
-// v_mfma_f32_16x16x32.
+// v_mfma_f32_16x16x32.  A sweep is those rows' way through the sequence's keys.
 //   - Only the device knows the lengths, so the workgroups divide the work
-//     there: the keys of all (sequence, head, 16 rows), in units of 128, lie in one
-//     line, of which each workgroup takes an equal piece, whatever the lengths and
-//     the table's room.  A piece that holds a whole sweep stores its result; the
-//     others leave partial results, two a workgroup at most, that a second kernel
-//     joins by their maxima and sums.
-//   - A wave takes 32 keys at a time, the next 32's K and V rows in flight in
-//     registers meanwhile.  The table's entries come from LDS, where they are
-//     laid once for many blocks: read from memory they would make each block wait for the
-//     loads before it, which come back in order.  32 lanes work out a row's
-//     address each and hand them on through LDS.
+//     there: the keys of all sequences lie in one line, in blocks of 32, which
+//     is cut into equal pieces, as many as let every (piece, head, tile of 16 rows) be a
+//     workgroup that runs at once, whatever the lengths and the table's room.  A piece
+//     that holds a whole sweep stores its result; the others leave partial results,
+//     two a workgroup at most, that a second kernel joins by their maxima and sums.
+//     Short tables take no pieces: eight waves a sweep, one launch (whole_sweeps).
+//   - The heads of a piece, whose rows lie side by side, run on one XCD and start a few
+//     workgroups apart: 8 sequences of 8 heads of 128 in e4m3 and 65536 positions 114 us;
+//     each head cut by itself 125, the heads side by side in order (all at the same line at
+//     once) 130.
+//   - A wave takes 32 keys at a time.  The next 32's K and V rows are under way in registers
+//     meanwhile, K's from where the scores have used K, V's from where the sums have used V:
+//     one set of registers, so that three workgroups of four waves fit a CU at 128 features
+//     (two: 131 us in the case above, four, spilling: 156).
+//   - Pages in sixteens (most): each half block lies in one page, whose entry and address
+//     are scalars and the row's offset the same for all blocks.  Other pages: the entries come from LDS, where
+//     they are laid once for many blocks (read from memory they would make each block wait for
+//     the loads before it, which come back in order); 32 lanes work out a row's address each and
+//     hand them on through LDS.
 //   - K rows are the A operand of S' = K Q', V rows transposed inside each lane
 //     (v_perm_b32) the A operand of O' += V' P', whose B operand the score
 //     registers are as they stand (keys 4 g + i and 16 + 4 g + i of lane group g
@@ -25,6 +34,10 @@
 //     largest weight where that is more), none of them 0 unless the weight is.
 //   - e4m3 becomes bf16 (v_cvt_scalef32_pk_bf16_fp8), exactly: 4 bits times a
 //     power of two; fp16 queries are then two bf16 parts, exactly.
+//
+// Bound by memory where there is enough of it: the case above reads 530 to 660 MB at 5.5 TB/s
+// (6.1 where a head's rows lie in a run); 16 sequences of 8 heads of 128 in bf16, 4096 positions at the
+// most, 170 MB in 36 us, 5 of them the join.  Short ones by the steps' latency, about 1.3 us each.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -63,8 +76,8 @@ struct PagedArgs {
   int64_t q_sh, q_ss, q_sb;
   int32_t seq, heads, kv_heads, batch, head_dim, causal, window;
   int32_t group, tiles, sweeps;  // query heads a cache head; tiles of 16 rows; sweeps a sequence
-  int32_t workers;               // workgroups
-  th::Divisor by_group, by_tiles, by_sweeps, by_workers;
+  int32_t shares;                // pieces of the line, at the most
+  th::Divisor by_group, by_tiles, by_sweeps, by_shares;
   float scale;
 };
 
@@ -109,26 +122,33 @@ __device__ __forceinline__ int running_sum(int x) {
   return x;
 }
 
-// The line of all sequences' blocks, sweep after sweep, and the piece of it that is this workgroup's:
-// 64 sequences at a time, a lane each.
+// The line of all sequences' blocks and the piece of it that is this workgroup's: 64
+// sequences at a time, a lane each.
 struct Line {
   Sequence own;            // lane's: sequence b0 + lane
   int end, b0;             // the line's length up to its end, from b0's start
-  int total, start, stop;  // the whole line; the piece
+  int share, start, stop;  // a piece's length; the piece
+  int piece, sweep;        // which one, and of which of each sequence's sweeps
   int b, before;           // a sequence, the line's length before it
 
   __device__ __forceinline__ int step(const PagedArgs& p, int at) {
     const int lane = threadIdx.x % 64;
     b0 = at;
     own = at + lane < p.batch ? sequence_of(p, at + lane) : Sequence{};
-    end = running_sum(own.blocks * p.sweeps);
+    end = running_sum(own.blocks);
     return __builtin_amdgcn_readlane(end, 63);
   }
   __device__ __forceinline__ bool find(const PagedArgs& p, int least) {
-    total = 0;
+    int total = 0;
     for (int at = 0; at < p.batch; at += 64) total += step(p, at);
-    const int share = max(least, thd::quotient(total + p.workers - 1, p.by_workers));
-    start = blockIdx.x * share, stop = min(total, start + share);
+    share = max(least, thd::quotient(total + p.shares - 1, p.by_shares));
+    // The sweeps of one piece are cache heads, whose rows lie side by side.  Pieces of a length
+    // worth it: piece by piece for the first sweep, then for the next, so that they start soon
+    // after each other, on one XCD where the pieces are in eights (workgroups go to the eight in
+    // turn).  Shortest pieces: those that have work come first.
+    if (share > least) sweep = thd::quotient(blockIdx.x, p.by_shares), piece = blockIdx.x - sweep * p.shares;
+    else piece = thd::quotient(blockIdx.x, p.by_sweeps), sweep = blockIdx.x - piece * p.sweeps;
+    start = piece * share, stop = min(total, start + share);
     if (start >= stop) return false;
     before = 0;
     if (p.batch > 64)
@@ -139,7 +159,7 @@ struct Line {
       }
     const int at = __ffsll((unsigned long long)__ballot(before + end > start)) - 1;
     b = b0 + at;
-    before += __builtin_amdgcn_readlane(end - own.blocks * p.sweeps, at);
+    before += __builtin_amdgcn_readlane(end - own.blocks, at);
     return true;
   }
   // Sequence b, or one after it.
@@ -192,7 +212,8 @@ struct Keys {
 // UNIFORM: pages in sixteens, so that each half block lies in one page.  The
 // wave reads its entry as a scalar, and the rows are at scalar addresses and
 // offsets that every block shares: no address is worked out on the vector ALU.
-// STREAM: V's loads are non-temporal (K's lines are each read by two loads).
+// STREAM: V's loads are non-temporal (16 sequences of 8 heads of 128 in bf16: 36 us, K's too, whose lines
+// are each read by two loads, 39).
 template <int D, int CT, bool EXACT, bool UNIFORM, bool STREAM>
 struct Block {
   static constexpr int E = D / 16;
@@ -377,7 +398,9 @@ __device__ __forceinline__ void split2_f16(float a, float b, uint32_t& w0, uint3
   w1 = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{ra, rb}, f16x2));
 }
 
-// Waves a SIMD that the registers are kept to.
+// Waves a SIMD that the registers are kept to: as many as keep a block's K and V and the sums without
+// spills (whole sweeps, whose eight waves need two, spill at 256 features and are still ahead there, 9.3 us
+// against 11.5 for 64 positions).
 constexpr int waves_of(int D, bool SINGLE, bool WHOLE) {
   if (WHOLE) return D > 64 || !SINGLE ? 2 : 4;
   return D > 128 ? 1 : D > 64 ? (SINGLE ? 3 : 2) : SINGLE ? 4 : 3;
@@ -434,40 +457,37 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
   const float c = p.scale * kLog2e;
   Line line;
   if constexpr (WHOLE) {
-    line.b = thd::quotient(blockIdx.x, p.by_sweeps);
-    line.before = line.b * p.sweeps;
+    line.b = thd::quotient(blockIdx.x, p.by_sweeps), line.sweep = blockIdx.x - line.b * p.sweeps;
     line.start = line.stop = 0;
   } else {
     if (!line.find(p, NW)) return;
   }
+  const int sweep = line.sweep, hk = thd::quotient(sweep, p.by_tiles), tile = sweep - hk * p.tiles;
   for (int u = line.start; WHOLE || u < line.stop;) {
     const int b = line.b;
-    int sweep, i0 = 0, i1, slot = -1;
+    int i0 = 0, i1, slot = -1;
     Sequence seq;
     if constexpr (WHOLE) {
       seq = sequence_of_all(p, b);
-      sweep = blockIdx.x - line.before;
       i1 = seq.blocks;
     } else {
       seq = line.sequence(p);
-      if (u - line.before >= seq.blocks * p.sweeps) {
-        line.before += seq.blocks * p.sweeps;
+      i0 = u - line.before;
+      if (i0 >= seq.blocks) {
+        line.before += seq.blocks;
         ++line.b;
         continue;
       }
-      sweep = (u - line.before) / seq.blocks, i0 = (u - line.before) - sweep * seq.blocks;
       i1 = min(seq.blocks, i0 + line.stop - u);
       const bool whole = i0 == 0 && i1 == seq.blocks;
-      slot = whole ? -1 : 2 * blockIdx.x + (u > line.start);
+      slot = whole ? -1 : 2 * (line.piece * p.sweeps + sweep) + (u > line.start);
       // Who has a sweep's first block says where its pieces are.
       if (i0 == 0 && threadIdx.x == 0) {
-        const int share = max(NW, thd::quotient(line.total + p.workers - 1, p.by_workers));
         int32_t* to = p.pieces + 2 * ((int64_t)b * p.sweeps + sweep);
-        to[0] = slot, to[1] = whole ? 0 : (u + seq.blocks - 1) / share - (int)blockIdx.x + 1;
+        to[0] = slot, to[1] = whole ? 0 : (u + seq.blocks - 1) / line.share - line.piece + 1;
       }
       u += i1 - i0;
     }
-    const int hk = thd::quotient(sweep, p.by_tiles), tile = sweep - hk * p.tiles;
     // The tile's rows are positions j0..j1 (position row / group, head row % group of the group).
     const int length = seq.length, count = seq.count;
     const int j0 = thd::quotient(kRows * tile, p.by_group);
@@ -747,7 +767,8 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
 
 // The rows whose sweep lies in several pieces, or has no keys: a workgroup for 64
 // features of a row, its threads in groups of 16, each of which takes every so
-// manieth piece, four loads at a time; then the groups' results in order.
+// manieth piece, four loads at a time; then the groups' results in order.  Bound by
+// latency: 4.8 us for 512 rows of 128 in about six pieces, 5.0 for 16 rows of 256 in 128.
 template <int D, bool F16>
 __global__ __launch_bounds__(1024) void paged_attn_join(PagedArgs p) {
   constexpr int slices = D / 64;
@@ -772,7 +793,7 @@ __global__ __launch_bounds__(1024) void paged_attn_join(PagedArgs p) {
       for (int i = 0; i < 4; ++i) {  // a piece past the last reads the last again, with no weight
         const int piece = min(i0 + i * groups, n - 1);
         // The first in either of its workgroup's places, the others in their first.
-        const int64_t from = (int64_t)(piece ? (at0 & ~1) + 2 * piece : at0) * kRows + row % kRows;
+        const int64_t from = (int64_t)(piece ? (at0 & ~1) + 2 * piece * p.sweeps : at0) * kRows + row % kRows;
         x[i] = reinterpret_cast<const f32x2*>(p.part_ml)[from];
         y[i] = *reinterpret_cast<const f32x4*>(p.part + from * D + f);
       }
@@ -855,22 +876,29 @@ int launch(const th_paged_desc* d, th_launch** out) {
   a.tiles = (int)(((int64_t)d->seq * a.group + kRows - 1) / kRows);
   a.sweeps = a.tiles * cache.heads;
   const int64_t keys = (int64_t)d->table_pages * cache.page, sweeps = (int64_t)a.sweeps * d->batch;
-  // As many workgroups as run at once, or as there are steps if that is fewer.
+  // As many workgroups as run at once (where that cuts the line in eight or more; otherwise four
+  // times as many, so that the last round counts for little), or as there are steps if that is fewer.
   const int64_t resident = (int64_t)th::ctx().prop.multiProcessorCount * waves_of(D, SINGLE, WHOLE);
-  a.workers = WHOLE ? (int)sweeps : (int)std::min(resident, sweeps * ((keys + NW * kBlock - 1) / (NW * kBlock)));
-  a.by_group = th::divisor(a.group), a.by_tiles = th::divisor(a.tiles), a.by_sweeps = th::divisor(a.sweeps);
-  a.by_workers = th::divisor(a.workers);
+  int64_t shares = resident / a.sweeps;
+  if (shares < 8) shares = (4 * resident + a.sweeps - 1) / a.sweeps;
+  if (shares >= 64) shares -= shares % 8;
+  shares = std::min(shares, d->batch * ((keys + NW * kBlock - 1) / (NW * kBlock)));
+  a.shares = (int)shares;
+  const int workers = WHOLE ? (int)sweeps : (int)(shares * a.sweeps);
+  a.by_group = th::divisor(a.group), a.by_tiles = th::divisor(a.tiles);
+  a.by_sweeps = th::divisor(a.sweeps), a.by_shares = th::divisor(a.shares);
   th::Builder b("attention_paged", 10);
-  const int k = b.kernel(fn, WHOLE ? "paged_attn_fwd_whole" : "paged_attn_fwd", dim3(a.workers), dim3(64 * NW), (uint32_t)lds, a);
+  const int k = b.kernel(fn, WHOLE ? "paged_attn_fwd_whole" : "paged_attn_fwd", dim3(workers), dim3(64 * NW), (uint32_t)lds, a);
   int end = k;
   if (!WHOLE) {
     // Threads for about as many pieces as a sweep has at the most.
     int threads = 256;
-    while (threads < 1024 && threads / 16 * 4 < a.workers / sweeps) threads *= 2;
+    while (threads < 1024 && threads / 16 * 4 < workers / sweeps) threads *= 2;
     end = b.kernel((const void*)paged_attn_join<D, F16>, "paged_attn_join", dim3(d->heads * (D / 64), d->seq, d->batch),
                    dim3(threads), 0, a);
-    const uint64_t at_o = b.workspace((uint64_t)a.workers * 2 * kRows * D * sizeof(float));
-    const uint64_t at_ml = b.workspace((uint64_t)a.workers * 2 * kRows * 2 * sizeof(float));
+    const uint64_t slots = a.shares > 1 ? 2 * (uint64_t)workers : 1;  // (one piece holds every sweep whole)
+    const uint64_t at_o = b.workspace(slots * kRows * D * sizeof(float));
+    const uint64_t at_ml = b.workspace(slots * kRows * 2 * sizeof(float));
     const uint64_t at_pieces = b.workspace((uint64_t)sweeps * 2 * sizeof(int32_t));
     for (int kk = k; kk <= end; ++kk) {
       b.ws_ref(kk, TH_OFFSET(PagedArgs, part), at_o);
@@ -894,7 +922,7 @@ int launch(const th_paged_desc* d, th_launch** out) {
   b.align(3, 16), b.align(4, 16);
   // All the cache there is room for: how much is held only the device knows.
   const double bytes = CT == kE4m3 ? 33.0 / 32 : 2, D0 = cache.head_dim, all = (double)d->batch * d->seq * d->heads;
-  b.work(2.0 * d->batch * cache.heads * (double)keys * D0 * bytes + 4.0 * all * D0, 4.0 * all * (double)keys * D0, a.workers);
+  b.work(2.0 * d->batch * cache.heads * (double)keys * D0 * bytes + 4.0 * all * D0, 4.0 * all * (double)keys * D0, workers);
   *out = b.release();
   return TH_OK;
 }

@@ -29,11 +29,11 @@ int build(const th_paged_desc* d, th_launch** out) {
              "paged attention: table, lengths, counts and lse must be 4-byte aligned");
   TH_REQUIRE(d->heads <= 65535 && d->seq <= 65535, "paged attention: heads and seq must be at most 65535");
   const int64_t rows = (int64_t)d->seq * (d->heads / d->cache.heads);
-  const int64_t keys = (int64_t)d->table_pages * d->cache.page, sweeps = (rows + 15) / 16 * d->cache.heads * d->batch;
+  const int64_t keys = (int64_t)d->table_pages * d->cache.page;
   TH_REQUIRE(rows <= 0x7fffffff - 16 && (int64_t)d->batch * d->seq * d->heads <= (1 << 22),
              "paged attention: batch * seq * heads must be at most 2^22");
-  TH_REQUIRE((double)sweeps * (double)((keys + 127) / 128 * 4) < 2147483647.0 - (1 << 20),
-             "paged attention: the table's room for all heads is too large");
+  TH_REQUIRE(d->batch * ((keys + 127) / 128 * 4) < 0x7fffffff - (1 << 20),
+             "paged attention: the table's room for all sequences is too large");
   if (int r = th::require_ready()) return r;
   const int n = d->cache.head_dim;
   return n <= 64 ? th::paged_attention_64(d, out) : n <= 128 ? th::paged_attention_128(d, out) : th::paged_attention_256(d, out);
