@@ -431,8 +431,11 @@ __device__ __forceinline__ uint32_t finite_of(uint32_t w) {
 }
 
 // EXACT: head_dim is D.  SINGLE: one new position a sequence, in one tile.  WHOLE: a workgroup of
-// eight waves a sweep, no pieces and nothing to join.
-template <int D, int CT, bool F16, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE>
+// eight waves a sweep, no pieces and nothing to join.  EARLY (WHOLE, entries by way of LDS, no window, so
+// that the keys start at 0): q, the table's entries and the first blocks' rows are asked for before the
+// lengths are here (what lies behind a length is some page's rows all the same): 421 positions in pages of
+// five 6.8 us to 6.2.  With scalar entries, which come as soon, 9.1 both ways for 600 positions.
+template <int D, int CT, bool F16, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE, bool EARLY>
 __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void paged_attn_fwd(PagedArgs p) {
   constexpr int E = D / 16;  // features of V a lane holds of each key
   constexpr int LD = D + 4;  // floats a row of a wave's O in LDS
@@ -466,6 +469,39 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
   for (int u = line.start; WHOLE || u < line.stop;) {
     const int b = line.b;
     int i0 = 0, i1, slot = -1;
+    // q's operands, a product's to each wave in turn: on their way here, in LDS behind the
+    // first block's loads.
+    constexpr int QN = (D / 32 + NW - 1) / NW;
+    u32x4 q[QN];
+    const int row = kRows * tile + r;
+    auto load_q = [&](bool there, int h, int j) {
+      const uint16_t* qrow = p.q + (int64_t)b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)j * p.q_ss;
+#pragma unroll
+      for (int n = 0; n < QN; ++n) {
+        const int s = wave + NW * n, f = CT == kE4m3 ? B::k_feature(s / 2, g) + 8 * (s % 2) : B::k_feature(s, g);
+        q[n] = there && s < D / 32 && (EXACT || f < p.head_dim) ? (u32x4) * reinterpret_cast<const u32x4_any*>(qrow + f) : u32x4{};
+      }
+    };
+    Keys keys{p.pages.table + (int64_t)p.pages.table_pages * b, entries, 0, p.pages.table_pages * p.pages.page - 1,
+              (int64_t)hk * p.pages.sh * B::bytes};
+    B x;
+    typename B::Rows rows;
+    typename B::Entries next;  // the next block's entries
+    // This wave's first block from s0: also where it has none before s1 (the last key's rows then),
+    // so that what waits for q below waits for no more.
+    auto begin = [&](int key0) {
+      next = B::look(p, keys, key0);
+      rows = x.load_k(p, keys, waves[wave], next, key0);
+      x.load_v(p, rows, waves[wave]);
+      next = B::look(p, keys, key0 + kStep);
+    };
+    if constexpr (EARLY) {
+      const int at = thd::quotient(row, p.by_group);
+      load_q(at < p.seq, hk * p.group + row - at * p.group, at);
+      for (int i = threadIdx.x; i < p.pages.table_pages; i += 64 * NW) entries[i] = keys.table[i];
+      __syncthreads();
+      begin(kBlock * wave);
+    }
     Sequence seq;
     if constexpr (WHOLE) {
       seq = sequence_of_all(p, b);
@@ -497,20 +533,11 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
     // Keys of this piece that any row sees, and those that every row sees.
     const int k_lo = max(seq.lo + kBlock * i0, first.lo / kBlock * kBlock), k_hi = j0 < count ? min(seq.lo + kBlock * i1, final.hi) : 0;
     const int all_lo = final.lo, all_hi = first.hi, last = final.hi - 1;
-    const int row = kRows * tile + r;
     const bool live = row < count * p.group;
     const int j = live ? thd::quotient(row, p.by_group) : j0, h = hk * p.group + (live ? row - j * p.group : 0);
     const Range mine = live ? seen_by(p, length, count, j) : Range{0, 0};
-    // q's operands, a product's to each wave in turn: on their way here, in LDS behind the
-    // first block's loads.
-    constexpr int QN = (D / 32 + NW - 1) / NW;
-    const uint16_t* qrow = p.q + (int64_t)b * p.q_sb + (int64_t)h * p.q_sh + (int64_t)j * p.q_ss;
-    u32x4 q[QN];
-#pragma unroll
-    for (int n = 0; n < QN; ++n) {
-      const int s = wave + NW * n, f = CT == kE4m3 ? B::k_feature(s / 2, g) + 8 * (s % 2) : B::k_feature(s, g);
-      q[n] = live && s < D / 32 && (EXACT || f < p.head_dim) ? (u32x4) * reinterpret_cast<const u32x4_any*>(qrow + f) : u32x4{};
-    }
+    if constexpr (!EARLY) load_q(live, h, j);
+    keys.last = last;
     auto lay_q = [&]() {
 #pragma unroll
       for (int n = 0; n < QN; ++n) {
@@ -535,13 +562,8 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = f32x4{};
     float m = -INFINITY, l = 0.0f;
-    Keys keys{p.pages.table + (int64_t)p.pages.table_pages * b, entries, 0, last,
-              (int64_t)hk * p.pages.sh * B::bytes};
     // The block of 32 keys from key0, the next one's loads (`more`) issued where its
     // operands' registers are free: K's after this one's scores, V's after its sums.
-    B x;
-    typename B::Rows rows;
-    typename B::Entries next;  // the next block's entries
     auto fold = [&](int key0, auto more) {
       Scales<D> sc;
       if constexpr (CT == kE4m3) sc.spread(waves[wave], x.scale, r, g);
@@ -680,22 +702,14 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
       __builtin_amdgcn_sched_barrier(0);
     };
     if (!WHOLE) __syncthreads();  // (the sweep before's results are read)
-    // This wave's first block from s0: also where it has none before s1 (the last key's rows then),
-    // so that what waits for q below waits for no more.
-    auto begin = [&](int key0) {
-      next = B::look(p, keys, key0);
-      rows = x.load_k(p, keys, waves[wave], next, key0);
-      x.load_v(p, rows, waves[wave]);
-      next = B::look(p, keys, key0 + kStep);
-    };
     auto go_on = [&](int key0, int s1) {
       if (key0 >= s1) return;
       for (; key0 + kStep < s1; key0 += kStep) fold(key0, std::true_type{});
       fold(key0, std::false_type{});
     };
-    if constexpr (UNIFORM) {
+    if constexpr (EARLY || UNIFORM) {
       if (k_lo < k_hi) {
-        begin(k_lo + kBlock * wave);
+        if constexpr (!EARLY) begin(k_lo + kBlock * wave);
         lay_q();
         __syncthreads();
         go_on(k_lo + kBlock * wave, k_hi);
@@ -852,14 +866,14 @@ inline bool whole_sweeps(const th_paged_desc* d) {
   return keys * row <= (sweeps < 64 ? 1 << 18 : 3 << 17);
 }
 
-template <int D, int CT, bool F16, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE>
+template <int D, int CT, bool F16, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE, bool EARLY>
 int launch(const th_paged_desc* d, th_launch** out) {
   constexpr int NW = WHOLE ? 8 : 4;
   constexpr size_t sweep_lds = (CT == kE4m3 && F16 ? 2 : 1) * kRows * D * 2 + NW * sizeof(WaveLds<D>) +
                                (UNIFORM ? 0 : kEntries * sizeof(int32_t));
   constexpr size_t result_lds = NW * kRows * (D + 4 + 2) * sizeof(float);
   constexpr size_t lds = sweep_lds > result_lds ? sweep_lds : result_lds;
-  const void* fn = (const void*)paged_attn_fwd<D, CT, F16, EXACT, UNIFORM, SINGLE, WHOLE>;
+  const void* fn = (const void*)paged_attn_fwd<D, CT, F16, EXACT, UNIFORM, SINGLE, WHOLE, EARLY>;
   if (lds > 65536) TH_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   const th_cache& cache = d->cache;
   PagedArgs a{};
@@ -927,19 +941,22 @@ int launch(const th_paged_desc* d, th_launch** out) {
   return TH_OK;
 }
 
-template <int D, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE>
+template <int D, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE, bool EARLY>
 int launch(const th_paged_desc* d, th_launch** out) {
-  if (d->cache.dtype == TH_BF16) return launch<D, kBf16, false, EXACT, UNIFORM, SINGLE, WHOLE>(d, out);
-  if (d->cache.dtype == TH_F16) return launch<D, kF16, true, EXACT, UNIFORM, SINGLE, WHOLE>(d, out);
-  return d->dtype == TH_F16 ? launch<D, kE4m3, true, EXACT, UNIFORM, SINGLE, WHOLE>(d, out)
-                            : launch<D, kE4m3, false, EXACT, UNIFORM, SINGLE, WHOLE>(d, out);
+  if (d->cache.dtype == TH_BF16) return launch<D, kBf16, false, EXACT, UNIFORM, SINGLE, WHOLE, EARLY>(d, out);
+  if (d->cache.dtype == TH_F16) return launch<D, kF16, true, EXACT, UNIFORM, SINGLE, WHOLE, EARLY>(d, out);
+  return d->dtype == TH_F16 ? launch<D, kE4m3, true, EXACT, UNIFORM, SINGLE, WHOLE, EARLY>(d, out)
+                            : launch<D, kE4m3, false, EXACT, UNIFORM, SINGLE, WHOLE, EARLY>(d, out);
 }
 template <int D, bool EXACT, bool UNIFORM, bool SINGLE>
 int launch(const th_paged_desc* d, th_launch** out) {
   // Whole sweeps of several positions of 256 features lack registers, the more with the
   // scalar addresses (12.5 us and 9.3 without, 2 x 64 positions of 8 heads in bf16).
   constexpr bool scalar = UNIFORM && (SINGLE || D < 256);
-  return whole_sweeps(d) ? launch<D, EXACT, scalar, SINGLE, true>(d, out) : launch<D, EXACT, UNIFORM, SINGLE, false>(d, out);
+  if (!whole_sweeps(d)) return launch<D, EXACT, UNIFORM, SINGLE, false, false>(d, out);
+  if constexpr (!scalar)
+    if (d->window == 0 && d->table_pages <= kEntries) return launch<D, EXACT, scalar, SINGLE, true, true>(d, out);
+  return launch<D, EXACT, scalar, SINGLE, true, false>(d, out);
 }
 // Pages in sixteens (and rows of a half block within 31 bits) take the scalar addresses.
 template <int D>

@@ -1,7 +1,7 @@
 // A key-value cache in pages: new rows written into it and held rows read
 // back, as they are (bf16, fp16) or as e4m3 codes with a scale of a power of two
 // for each 32 features.  Memory-bound: each row is read once and written once
-// (16 contexts of 8192 positions at the most, 8 heads of 128, from e4m3: 89 us, 5.2 TB/s; single
+// (8 contexts of 16384 positions at the most, 8 heads of 128, from e4m3: 89 us, 5.2 TB/s; single
 // positions 2.4 us, the launch).
 //
 // A thread moves 8 features of K and the same 8 of V (16 bytes of each on the dense side),

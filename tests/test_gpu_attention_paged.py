@@ -153,6 +153,36 @@ def test_the_widest_windows(target, page, cap, window):
     _check(c, q, o, lse, n, m, was=6.0, window=window)
 
 
+@pytest.mark.parametrize("S,KV,cap", [(1, 700, 3600), (3, 300, 3600), (1, 4100, 3600)])
+def test_more_sweeps_than_workgroups_at_once(target, S, KV, cap):
+    """The keys in few pieces, down to one, that holds every sweep whole."""
+    announce("paged many heads", S, KV, cap)
+    B, D, page = 3, 8, 16
+    c = Paged(B, cap, KV, D, page, "bf16", False)
+    gen = torch.Generator(device="cuda").manual_seed(KV)
+    _fill(c, gen, cap)
+    q = rows(gen, "bf16", B, S, KV, D, spread=False)
+    lengths = [cap, 0, 2077]
+    n = ints(*lengths)
+    o, lse = torch.full_like(q, 6.0), torch.full((B, S, KV), 6.0, device="cuda")
+    _attend(c, q, o, lse, n)()
+    torch.cuda.synchronize()
+    assert (o[1] == 0).all() and torch.isneginf(lse[1]).all()
+    for b in (0, 2):
+        k, v = (t[c.table[b].long()].reshape(-1, KV, D)[:lengths[b]].double() for t in (c.k, c.v))
+        for j in range(S):
+            seen = lengths[b] - S + j + 1
+            s = (k[:seen] * q[b, j].double()).sum(-1) * D ** -0.5
+            w = torch.softmax(s, 0)
+            want = torch.stack([(w * v[:seen, :, d]).sum(0) for d in range(D)], -1)
+            score = (q[b, j].double().abs() * k.abs().amax(0)).sum(-1) * D ** -0.5 * ((D + 8) * 2.0 ** -24 + 2.0 ** -22)
+            rel = 2 * (score + 2.0 ** -21 + (seen / 128 + 40) * 2.0 ** -24)
+            limit = rel[:, None] * v.abs().amax(0) + 2.0 ** -8 * want.abs() + 2.0 ** -25
+            assert ((o[b, j].double() - want).abs() <= limit).all()
+            exact = torch.logsumexp(s, 0)
+            assert ((lse[b, j].double() - exact).abs() <= score + 2.0 ** -20 + 2.0 ** -22 * exact.abs()).all()
+
+
 @pytest.mark.parametrize("S,page,cap,e4m3", [(1, 16, 200, False), (5, 7, 200, True), (1, 7, 6000, True), (9, 16, 3000, False)])
 def test_over_its_queries(target, S, page, cap, e4m3):
     announce("paged in place", S, page, cap, e4m3)
