@@ -233,8 +233,10 @@ bool rows_apart(int64_t row, const int64_t* strides, const int64_t* extents, int
   std::sort(order, order + m, [&](int a, int b) { return strides[a] < strides[b]; });
   int64_t span = row;
   for (int i = 0; i < m; ++i) {
-    if (strides[order[i]] < span) return false;
-    span += strides[order[i]] * (extents[order[i]] - 1);
+    int64_t more;  // (an extent whose bytes pass 64 bits is taken as overlapping)
+    if (strides[order[i]] < span || __builtin_mul_overflow(strides[order[i]], extents[order[i]] - 1, &more) ||
+        __builtin_add_overflow(span, more, &span) || span > (int64_t)1 << 60)
+      return false;
   }
   return true;
 }

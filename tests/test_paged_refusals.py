@@ -55,7 +55,7 @@ BAD_CACHES = [dict(dtype=L.F32), dict(head_dim=60), dict(head_dim=264), dict(hea
               dict(pages=0), dict(page=1 << 16, pages=1 << 15), dict(k=0), dict(v=P + 8), dict(dtype=L.E4M3),
               dict(dtype=L.E4M3, k_scales=P, v_scales=P, head_dim=80), dict(dtype=L.E4M3, k_scales=P, v_scales=P + 2), dict(strides=(64, 100, 2048)),
               dict(strides=(64, -128, 2048)), dict(strides=(64, 64, 2048)), dict(strides=(64, 128, 1024)),
-              dict(**E4M3, strides=(80, 160, 2560))]
+              dict(**E4M3, strides=(80, 160, 2560)), dict(strides=(64, 128, 1 << 61)), dict(strides=(1 << 62, 64, 2048))]
 
 
 @pytest.mark.parametrize("bad", BAD_CACHES, ids=str)
