@@ -142,6 +142,10 @@ struct Line {
     int total = 0;
     for (int at = 0; at < p.batch; at += 64) total += step(p, at);
     share = max(least, thd::quotient(total + p.shares - 1, p.by_shares));
+    // A second step that only some waves take lasts as long as a full one, and fewer pieces are
+    // joined: 2 sequences of one head of 256, five blocks a piece 19.9 us, eight 17.5.  (Longer pieces
+    // lose more workgroups than they gain: nine to twelve, 17.5 us to 18.1.)
+    if (share < 2 * least) share = (share + least - 1) & -least;
     // The sweeps of one piece are cache heads, whose rows lie side by side.  Pieces of a length
     // worth it: piece by piece for the first sweep, then for the next, so that they start soon
     // after each other, on one XCD where the pieces are in eights (workgroups go to the eight in
@@ -782,7 +786,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
 // The rows whose sweep lies in several pieces, or has no keys: a workgroup for 64
 // features of a row, its threads in groups of 16, each of which takes every so
 // manieth piece, four loads at a time; then the groups' results in order.  Bound by
-// latency: 4.8 us for 512 rows of 128 in about six pieces, 5.0 for 16 rows of 256 in 128.
+// latency: 4.8 us for 512 rows of 128 in about six pieces, 5.0 for 16 rows of 256 in 72.
 template <int D, bool F16>
 __global__ __launch_bounds__(1024) void paged_attn_join(PagedArgs p) {
   constexpr int slices = D / 64;
