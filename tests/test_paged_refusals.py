@@ -82,9 +82,14 @@ def test_a_cache_every_kernel_takes(f, good):
     (_attend, dict(window=5, causal=False)), (_attend, dict(q=0)), (_attend, dict(o=P + 1)),
     (_attend, dict(q_strides=(64, 0, 128))), (_attend, dict(q_strides=(64, 256, -1))), (_attend, dict(table=0)),
     (_attend, dict(lengths=0)), (_attend, dict(seq=0)), (_attend, dict(batch=0)),
-    (_attend, dict(seq=1 << 20, batch=1, q_strides=(64, 256, 0))), (_attend, dict(batch=65535, seq=200))], ids=str)
+    (_attend, dict(seq=1 << 20, batch=1, q_strides=(64, 256, 0))), (_attend, dict(batch=65535, seq=200)),
+    (_attend, dict(batch=64, table_pages=1 << 26))], ids=str)
 def test_arguments_no_kernel_takes(f, bad):
     assert _code(f, **bad) == ARGUMENT
+
+
+def test_the_largest_tables():
+    assert _code(_attend, batch=32, table_pages=1 << 26) == STATE
 
 
 @pytest.mark.parametrize("f", [_write, _read, _attend])
