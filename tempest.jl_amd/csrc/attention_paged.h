@@ -857,17 +857,19 @@ __global__ __launch_bounds__(1024) void paged_attn_join(PagedArgs p) {
 }
 
 // Whether each sweep is one workgroup's, nothing joined: a launch and its waits less, but a
-// step's bytes go through one CU (about 1.3 us for 256 keys of 256 bytes).  Both measured, 32/8
-// heads of 128 in bf16, tables of 400, 800 and 1400 positions: one sequence 7.8, 10.6 and
-// 15.9 us whole, 10.5, 10.4 and 10.5 in pieces; 64 sequences 16, 31 and 51, and 24, 32
-// and 48.  The row's bytes weigh as the border of 64, 128 and 256 features says (1200, 750 and
-// 400 positions in bf16 for few sweeps, half as many again for 64 or more; e4m3 1400, 900, 550).
+// step's bytes go through one CU (about 1.3 us for 256 keys of 256 bytes), and what is left over of a
+// round of workgroups waits.  Both measured, whole and in pieces, 32/8 heads of 128 in bf16: one
+// sequence and a table of 500 positions 8.8 and 9.0 us, of 1000 12.7 and 10.0; 24 sequences (192 sweeps, a CU
+// each) of 850 13.7 and 18.1, of 1400 21.5 and 22.6; 64 sequences of 750 28.6 and 30.7, of
+// 1000 38.7 and 34.9.  The row's bytes weigh as the borders of 64, 128 and 256 features say (few
+// sweeps 1000, 650 and 370 positions in bf16, 800 of 128 in e4m3; a CU each 2300, 1500 and 850, 1800).
 inline bool whole_sweeps(const th_paged_desc* d) {
   int64_t keys = (int64_t)d->table_pages * d->cache.page;
   if (d->window > 0) keys = std::min<int64_t>(keys, (int64_t)d->window + d->seq + 2 * kBlock);
   const int64_t sweeps = ((int64_t)d->seq * (d->heads / d->cache.heads) + kRows - 1) / kRows * d->cache.heads * d->batch;
   const int64_t row = 96 + d->cache.head_dim * (d->cache.dtype == TH_E4M3 ? 3 : 4) / 2;
-  return keys * row <= (sweeps < 64 ? 1 << 18 : 3 << 17);
+  const int64_t cus = th::ctx().prop.multiProcessorCount;
+  return keys * row <= (8 * sweeps < 3 * cus ? 7 << 15 : sweeps <= cus ? 1 << 19 : 9 << 15);
 }
 
 template <int D, int CT, bool F16, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE, bool EARLY>

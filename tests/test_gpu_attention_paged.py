@@ -103,6 +103,7 @@ CASES = [  # B, S, H, KV, D, page, cap, dtype, e4m3, outer, lengths, counts, mas
     (1, 1, 8, 8, 64, 64, 9000, "bf16", True, False, [8999], None, {"scale": 0.3}),
     # Long tables: the keys divided among workgroups, pieces joined.
     (150, 1, 4, 1, 64, 64, 1600, "bf16", False, False, [(211 * i) % 1601 if i % 3 else 0 for i in range(150)], None, {}),
+    (150, 1, 4, 1, 64, 64, 2600, "bf16", False, False, [(211 * i) % 2601 if i % 3 else 0 for i in range(150)], None, {}),
     (70, 2, 2, 1, 64, 7, 1500, "f16", True, False, [(97 * i) % 1501 for i in range(70)], [i % 3 for i in range(70)], {}),
     (3, 1, 16, 2, 256, 16, 1200, "f16", False, True, [1200, 0, 33], None, {}),
     (2, 3, 6, 2, 256, 32, 1000, "bf16", True, False, [1000, 999], [3, 2], {}),
