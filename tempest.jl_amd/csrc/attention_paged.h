@@ -863,13 +863,15 @@ __global__ __launch_bounds__(1024) void paged_attn_join(PagedArgs p) {
 // each) of 850 13.7 and 18.1, of 1400 21.5 and 22.6; 64 sequences of 750 28.6 and 30.7, of
 // 1000 38.7 and 34.9.  The row's bytes weigh as the borders of 64, 128 and 256 features say (few
 // sweeps 1000, 650 and 370 positions in bf16, 800 of 128 in e4m3; a CU each 2300, 1500 and 850, 1800).
+// Few sweeps in pages not in sixteens, whose pieces take longer to start: one sequence of 750, pages of
+// five, 10.6 whole and 10.7; proposals of 12/4 heads of 64 in a window of 1000, pages of seven, 11.3 and 13.2.
 inline bool whole_sweeps(const th_paged_desc* d) {
   int64_t keys = (int64_t)d->table_pages * d->cache.page;
   if (d->window > 0) keys = std::min<int64_t>(keys, (int64_t)d->window + d->seq + 2 * kBlock);
   const int64_t sweeps = ((int64_t)d->seq * (d->heads / d->cache.heads) + kRows - 1) / kRows * d->cache.heads * d->batch;
   const int64_t row = 96 + d->cache.head_dim * (d->cache.dtype == TH_E4M3 ? 3 : 4) / 2;
   const int64_t cus = th::ctx().prop.multiProcessorCount;
-  return keys * row <= (8 * sweeps < 3 * cus ? 7 << 15 : sweeps <= cus ? 1 << 19 : 9 << 15);
+  return keys * row <= (8 * sweeps < 3 * cus ? (d->cache.page % 16 ? 1 << 18 : 7 << 15) : sweeps <= cus ? 1 << 19 : 9 << 15);
 }
 
 template <int D, int CT, bool F16, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE, bool EARLY>
