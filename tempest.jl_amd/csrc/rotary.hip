@@ -37,9 +37,16 @@ struct RotaryArgs {
   int32_t turning, passing;      // items of a head: turned, copied
   int32_t pass_second;           // features from a copied item's first vector to its second (0: it has one)
   int32_t per_block;             // tokens a workgroup
-  th::Divisor by_seq, by_half, by_token, by_head;  // (items of a token, of a head)
+  th::Divisor by_seq, by_half;
+  th::Divisor by_token[2], by_head[2];  // items of a token, of a head: turned alone, copied too
   float sign;
 };
+
+// Whether what passes has to be copied: an array's result lies elsewhere.  The
+// kernel asks, for the arrays may be pointed elsewhere after the launch was built.
+__host__ __device__ __forceinline__ bool moves(const RotaryArray& q, const RotaryArray& k) {
+  return q.x != q.y || (k.heads && k.x != k.y);
+}
 
 // sin and cos of 2 pi t.
 __device__ __forceinline__ float2 turned(double t) {
@@ -115,20 +122,22 @@ __global__ __launch_bounds__(256) void rotary(RotaryArgs p) {
   typedef Vec<E, V> W;
   extern __shared__ float2 turns[];  // [token][pair]: sin, cos
   const int first = blockIdx.x * p.per_block, tokens = min(p.per_block, p.tokens - first);
-  const int per_head = p.turning + p.passing;
-  const int per_token = (p.a[0].heads + p.a[1].heads) * per_head, items = tokens * per_token;
+  const RotaryArray qa = p.a[0], ka = p.a[1];
+  const bool copy = moves(qa, ka);
+  const th::Divisor by_token = p.by_token[copy], by_head = p.by_head[copy];
+  const int per_head = p.turning + (copy ? p.passing : 0);
+  const int per_token = (qa.heads + ka.heads) * per_head, items = tokens * per_token;
   // An item's place: its token of the workgroup's, its features of x and y.
   struct Item {
     const E* x;
     E* y;
     int t, item, f0, f1;
   };
-  const RotaryArray qa = p.a[0], ka = p.a[1];
   auto item_of = [&](int i) {
     Item it;
-    it.t = thd::quotient(i, p.by_token);
+    it.t = thd::quotient(i, by_token);
     const int at = i - it.t * per_token;
-    int head = thd::quotient(at, p.by_head);
+    int head = thd::quotient(at, by_head);
     it.item = at - head * per_head;
     const bool second = head >= qa.heads;
     auto of = [&](auto q, auto k) { return second ? k : q; };  // (scalars both, not loads from where the index says)
@@ -255,18 +264,22 @@ int build(const th_rotary_desc* d, th_launch** out) {
   int v = 16 / size;
   while (half % v || pass % v) v /= 2;
   const bool pairs = d->flags & TH_ROTARY_PAIRS;
-  const bool copy = pass && !(d->q_out == d->q && (!d->kv_heads || d->k_out == d->k));
   a.turning = half / v, a.pass_second = pass % (2 * v) == 0 ? v : 0;
-  a.passing = copy ? pass / (v + a.pass_second) : 0;
-  const int64_t per_token = (int64_t)(d->heads + d->kv_heads) * (a.turning + a.passing);
+  a.passing = pass / (v + a.pass_second);
+  // The workgroups are sized for where the arrays lie now; any share of the items is right.
+  const int all = d->heads + d->kv_heads;
+  const int64_t per_token = (int64_t)all * (a.turning + (moves(a.a[0], a.a[1]) ? a.passing : 0));
   TH_REQUIRE(per_token <= (1 << 24), "rotary: heads * head_dim is too large");
   // About four items a thread, at most 8 KB of angles.
   a.per_block = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / per_token, 1024 / half));
   const int64_t blocks = (tokens + a.per_block - 1) / a.per_block;
   TH_REQUIRE(blocks <= 0xffffff, "rotary: batch * seq is too large");  // 2^32 threads
   if (int r = th::require_ready()) return r;
-  a.by_seq = th::divisor(a.seq), a.by_half = th::divisor(a.half), a.by_token = th::divisor((int)per_token);
-  a.by_head = th::divisor(a.turning + a.passing);
+  a.by_seq = th::divisor(a.seq), a.by_half = th::divisor(a.half);
+  for (int copy = 0; copy < 2; ++copy) {
+    const int per_head = a.turning + copy * a.passing;
+    a.by_head[copy] = th::divisor(per_head), a.by_token[copy] = th::divisor(all * per_head);
+  }
   const void* fn = d->dtype == TH_F32    ? kernel_of<TH_F32>(v, pairs)
                    : d->dtype == TH_BF16 ? kernel_of<TH_BF16>(v, pairs)
                                          : kernel_of<TH_F16>(v, pairs);

@@ -159,3 +159,57 @@ def test_rotary_gradient_of_a_graph(target):
     fwd()
     torch.cuda.synchronize()
     _check(yq, q2, positions, freqs, [32], False, False, "f32")
+
+
+@pytest.mark.parametrize("dtype,D,R,H,KV,pairs", [("bf16", 64, 32, 4, 2, False), ("f32", 80, 20, 3, 0, True),
+                                                  ("f16", 7, 6, 2, 1, True), ("bf16", 256, 64, 40, 8, False)])
+def test_rotary_moves_between_in_place_and_apart(target, dtype, D, R, H, KV, pairs):
+    """Built in place with part of a head turned, then pointed at another q_out and k_out, at another
+    q and k, and back: the features that pass are in every result.  And built apart, then in place."""
+    import tempest_hip.launch as L
+    announce("rotary moves", dtype, D, R, H, KV, pairs)
+    B, S = 2, 37
+    gen = torch.Generator(device="cuda").manual_seed(D + R)
+    dt = TYPES[dtype]
+    x = {"q": _array(gen, dt, B, S, H, D), "k": _array(gen, dt, B, S, max(KV, 1), D)}
+    positions = torch.randint(0, 1 << 16, (B, S, 1), dtype=torch.int32, device="cuda", generator=gen)
+    freqs = _freqs(R // 2)
+
+    def launch(a, y):
+        return L.rotary(B, S, H, KV, D, a["q"].data_ptr(), a["k"].data_ptr(), y["q"].data_ptr(), y["k"].data_ptr(),
+                        positions.data_ptr(), freqs.data_ptr(), rotary_dim=R, pairs=pairs, dtype=_dtype(dtype))
+
+    def held(y):
+        torch.cuda.synchronize()
+        for n in ("q", "k") if KV else ("q",):
+            _check(y[n], x[n], positions, freqs, [R // 2], pairs, False, dtype)
+
+    def copies():
+        return {n: t.clone() for n, t in x.items()}
+
+    def empty():
+        return {n: torch.full_like(t, 7.0) for n, t in x.items()}
+    a = copies()
+    f = launch(a, a)
+    f()
+    held(a)
+    a, y = copies(), empty()
+    for n in ("q", "k"):
+        f.repoint(n, a[n].data_ptr())
+        f.repoint(n + "_out", y[n].data_ptr())
+    f()
+    held(y)
+    assert torch.equal(a["q"], x["q"]) and torch.equal(a["k"], x["k"])
+    b = copies()  # q and k elsewhere, where one stays in place: both results whole
+    f.repoint("q_out", a["q"].data_ptr())
+    f.repoint("k", b["k"].data_ptr())
+    y["k"].fill_(7.0)
+    f()
+    held({"q": a["q"], "k": y["k"]})
+    a, y = copies(), empty()
+    g = launch(a, y)
+    for n in ("q", "k"):
+        g.repoint(n + "_out", a[n].data_ptr())
+    g()
+    held(a)
+    assert (y["q"] == 7.0).all() and (y["k"] == 7.0).all()
