@@ -858,8 +858,8 @@ int th_build_cache_read(const th_cache_desc* desc, th_launch** host_out);
  * type or beside TH_E4M3; any alignment; o may be q.  lse (if non-NULL) as th_build_attention_fwd
  * writes it; heads a multiple of the cache's heads; batch * seq * heads at most 2^22,
  * batch * table_pages * page at most 2^35; scale <= 0 means 1/sqrt(head_dim).
- * The weights are fp32's, as are all sums.  The keys are read once for every 16 rows
- * (seq * heads / cache heads).  Workspace: the split's partial results.
+ * The weights are fp32's (over an fp16 cache to 22 bits each, however small), as are all sums.  The keys
+ * are read once for every 16 rows (seq * heads / cache heads).  Workspace: the split's partial results.
  * Values: 0 q, 1 o, 2 lse, 3 the cache's k, 4 its v, 5 k_scales, 6 v_scales,
  * 7 table, 8 lengths, 9 counts. */
 typedef struct th_paged_desc {

@@ -29,9 +29,12 @@
 //     (v_perm_b32) the A operand of O' += V' P', whose B operand the score
 //     registers are as they stand (keys 4 g + i and 16 + 4 g + i of lane group g
 //     being slots i and 4 + i).
-//   - The weights are fp32's: three bf16 parts (split2_towards0), or for fp16
-//     values two fp16 parts of 2^15 times the weight (22 bits, and 2^-39 of the
-//     largest weight where that is more), none of them 0 unless the weight is.
+//   - The weights are fp32's: three bf16 parts (split2_towards0), none of them 0 unless
+//     the weight is.  Beside fp16 values, two fp16 parts of 2^15 times the weight (22 bits, half of what
+//     the exponential leaves open) in the blocks where no weight is under 2^-16 of the largest so far, for
+//     fp16 ends at 2^-39 of it; in the others three bf16 parts, and the values as two, exactly.  16 sequences
+//     of 8 heads of 128 in fp16 38.7 us, 40.8 where all blocks hold small weights (fp16 parts alone 36.0, and
+//     weights under 2^-38 wrong; bf16 parts alone 39.9, and one sequence of 600 positions 11.0 for 9.5).
 //   - e4m3 becomes bf16 (v_cvt_scalef32_pk_bf16_fp8), exactly: 4 bits times a
 //     power of two; fp16 queries are then two bf16 parts, exactly.
 //
@@ -392,22 +395,36 @@ __device__ __forceinline__ uint32_t rounded2(float a, float b) {
   return pack2(a, b);
 }
 
-// x >= 0 (at most 2^15) in two fp16 parts, 22 bits or 2^-24, the first towards
-// 0 and neither 0 unless x is: an infinite value they multiply stays one.
+// x in 2^-1..2^15, or 0, in two fp16 parts, 22 bits, the first towards 0 and neither 0 unless x is: an
+// infinite value they multiply stays one.
 __device__ __forceinline__ void split2_f16(float a, float b, uint32_t& w0, uint32_t& w1) {
   const float least = 5.9604645e-8f;  // fp16's least, 2^-24
-  const auto hi = __builtin_amdgcn_cvt_pkrtz(a > 0 ? fmaxf(a - least, least) : 0.0f, b > 0 ? fmaxf(b - least, least) : 0.0f);
+  const auto hi = __builtin_amdgcn_cvt_pkrtz(fmaxf(a - least, 0.0f), fmaxf(b - least, 0.0f));
   const float ra = a > 0 ? fmaxf(a - (float)hi[0], least) : 0.0f, rb = b > 0 ? fmaxf(b - (float)hi[1], least) : 0.0f;
   w0 = __builtin_bit_cast(uint32_t, hi);
   w1 = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{ra, rb}, f16x2));
 }
 
+// Two words of fp16 pairs (two features of two keys) as bf16 pairs of each feature: the top 8 bits of its
+// 11, and the other 3, exactly.  An infinity is the first part's; the second is then finite (an
+// infinity less itself is NaN, which fmaxf drops; no part that is a number reaches -256).
+__device__ __forceinline__ void split_f16(uint32_t key0, uint32_t key1, uint32_t (&even)[2], uint32_t (&odd)[2]) {
+  const f32x2 a = __builtin_convertvector(__builtin_bit_cast(f16x2, key0), f32x2);
+  const f32x2 b = __builtin_convertvector(__builtin_bit_cast(f16x2, key1), f32x2);
+  auto top = [](float x) { return __float_as_uint(x) & 0xffff0000u; };
+  auto rest = [&](float x) { return __float_as_uint(fmaxf(x - __uint_as_float(top(x)), -256.0f)); };
+  auto high = [](uint32_t x, uint32_t y) { return __builtin_amdgcn_perm(y, x, 0x07060302u); };
+  even[0] = high(__float_as_uint(a[0]), __float_as_uint(b[0])), even[1] = high(rest(a[0]), rest(b[0]));
+  odd[0] = high(__float_as_uint(a[1]), __float_as_uint(b[1])), odd[1] = high(rest(a[1]), rest(b[1]));
+}
+
 // Waves a SIMD that the registers are kept to: as many as keep a block's K and V and the sums without
 // spills (whole sweeps, whose eight waves need two, spill at 256 features and are still ahead there, 9.3 us
-// against 11.5 for 64 positions).
-constexpr int waves_of(int D, bool SINGLE, bool WHOLE) {
+// against 11.5 for 64 positions).  fp16's two ways of the sums need more: with one more wave 16 sequences of 8
+// heads of 128 take 39.2 us for 38.7, 46.4 for 40.8 where weights are small.
+constexpr int waves_of(int D, int CT, bool SINGLE, bool WHOLE) {
   if (WHOLE) return D > 64 || !SINGLE ? 2 : 4;
-  return D > 128 ? 1 : D > 64 ? (SINGLE ? 3 : 2) : SINGLE ? 4 : 3;
+  return D > 128 ? 1 : (D > 64 ? 2 : 3) + (SINGLE && CT != kF16);
 }
 
 // Whether one of a word's values is NaN or an infinity.
@@ -440,15 +457,14 @@ __device__ __forceinline__ uint32_t finite_of(uint32_t w) {
 // lengths are here (what lies behind a length is some page's rows all the same): 421 positions in pages of
 // five 6.8 us to 6.2.  With scalar entries, which come as soon, 9.1 both ways for 600 positions.
 template <int D, int CT, bool F16, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE, bool EARLY>
-__global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void paged_attn_fwd(PagedArgs p) {
+__global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, CT, SINGLE, WHOLE)) void paged_attn_fwd(PagedArgs p) {
   constexpr int E = D / 16;  // features of V a lane holds of each key
   constexpr int LD = D + 4;  // floats a row of a wave's O in LDS
   constexpr int NW = WHOLE ? 8 : 4;               // waves
   constexpr int kStep = kBlock * NW;              // keys they take at a time
-  constexpr bool kHalf = CT == kF16;              // products in fp16, not bf16
+  constexpr bool kHalf = CT == kF16;              // scores, and most weighted sums, in fp16, not bf16
   constexpr int QP = CT == kE4m3 && F16 ? 2 : 1;  // parts of q
-  constexpr int WP = kHalf ? 2 : 3;               // parts of a weight
-  constexpr float kBias = kHalf ? 15.0f : 0.0f;   // weights are held times 2^kBias
+  constexpr float kTimes = kHalf ? 32768.0f : 1.0f;  // o is held times this
   typedef Block<D, CT, EXACT, UNIFORM, SINGLE && !WHOLE> B;
   // LDS holds q's operands, what a wave shares with itself and the table's entries while a
   // sweep runs, then the waves' results.
@@ -597,13 +613,20 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
       // see them by themselves.
       uint32_t differ = 0;  // bit i: some rows see the lane's key i, some do not
       bool apart = false;
+      float low = INFINITY;  // fp16: the least score that the lane's row sees, but NaN
+      if constexpr (kHalf)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) low = fminf(low, s[i / 4][i % 4]);
       if (!(key0 >= all_lo && key0 + kBlock <= all_hi && present == 0xffffffffu)) {
         uint32_t strange = 0;
+        low = INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int n = 16 * (i / 4) + 4 * g + i % 4, key = key0 + n;
           const bool held = present >> n & 1, some = held && key >= first.lo && key < final.hi;
-          s[i / 4][i % 4] = held && key >= mine.lo && key < mine.hi ? s[i / 4][i % 4] : -INFINITY;
+          const bool seen = held && key >= mine.lo && key < mine.hi;
+          if constexpr (kHalf) low = seen ? fminf(low, s[i / 4][i % 4]) : low;
+          s[i / 4][i % 4] = seen ? s[i / 4][i % 4] : -INFINITY;
           if constexpr (CT == kE4m3) sc.v[i] = some ? sc.v[i] : 1.0f;
           if constexpr (SINGLE) {
 #pragma unroll
@@ -635,21 +658,15 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
         for (int e = 0; e < E; ++e) o[e] *= alpha;
         m = mn;
       }
-      u32x4 wp[WP];
       float w[8];
+      auto weights = [&]() {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], c, kBias - shift));
-        l += w[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t a, b2, d2 = 0;
-        if constexpr (kHalf) split2_f16(w[2 * i], w[2 * i + 1], a, b2);
-        else split2_towards0(w[2 * i], w[2 * i + 1], a, b2, d2);
-        wp[0][i] = a, wp[1][i] = b2;
-        if constexpr (WP == 3) wp[2][i] = d2;
-      }
+        for (int i = 0; i < 8; ++i) {
+          w[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], c, -shift));
+          l += w[i];
+        }
+      };
+      if constexpr (!kHalf) weights();
       auto value = [&](int i, int d2) {  // features 2 d2 and 2 d2 + 1 of the lane's key i
         if constexpr (CT == kE4m3) return bf16_of(x.v[i][d2 / 2], sc.v[i], d2 % 2);
         else return x.v[i][d2];
@@ -657,8 +674,9 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
       if (apart) {
         constexpr uint32_t one = kHalf ? 0x3c00u : 0x3f80u, top = kHalf ? 0x7c00u : 0x7f80u;
         u32x4 sees;  // 1 for each key of the row's
+        auto seen_weight = [&](int i) { return kHalf ? __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], c, -shift)) : w[i]; };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sees[i] = (w[2 * i] > 0 ? one : 0u) | (w[2 * i + 1] > 0 ? one << 16 : 0u);
+        for (int i = 0; i < 4; ++i) sees[i] = (seen_weight(2 * i) > 0 ? one : 0u) | (seen_weight(2 * i + 1) > 0 ? one << 16 : 0u);
 #pragma unroll
         for (int d = 0; d < E; ++d)
 #pragma unroll 1
@@ -685,24 +703,57 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
           if (whole && (differ >> i & 1)) sc.v[i] = 1.0f;
         }
       }
-#pragma unroll
-      for (int d2 = 0; d2 < E / 2; ++d2) {
-        uint32_t v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = value(i, d2);
-        u32x4 even, odd;  // the two features of the eight keys
+      // o += V' P', in fp16 or in bf16.
+      auto sums = [&](auto half) {
+        constexpr int WP = half ? 2 : 3, VP = kHalf && !half ? 2 : 1;  // parts of a weight, of a value
+        u32x4 wp[WP];
+        if constexpr (kHalf) weights();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          even[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x05040100u);
-          odd[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x07060302u);
+          uint32_t a, b2, d2 = 0;
+          if constexpr (half) split2_f16(w[2 * i] * kTimes, w[2 * i + 1] * kTimes, a, b2);
+          else split2_towards0(w[2 * i] * kTimes, w[2 * i + 1] * kTimes, a, b2, d2);
+          wp[0][i] = a, wp[1][i] = b2;
+          if constexpr (WP == 3) wp[2][i] = d2;
         }
 #pragma unroll
-        for (int z = WP - 1; z >= 0; --z) {
-          o[2 * d2] = product<kHalf>(even, wp[z], o[2 * d2]);
-          o[2 * d2 + 1] = product<kHalf>(odd, wp[z], o[2 * d2 + 1]);
+        for (int d2 = 0; d2 < E / 2; ++d2) {
+          uint32_t v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = value(i, d2);
+          u32x4 even[VP], odd[VP];  // the two features of the eight keys
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (VP == 2) {
+              uint32_t e[2], f[2];
+              split_f16(v[2 * i], v[2 * i + 1], e, f);
+              even[0][i] = e[0], even[1][i] = e[1], odd[0][i] = f[0], odd[1][i] = f[1];
+            } else {
+              even[0][i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x05040100u);
+              odd[0][i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x07060302u);
+            }
+          }
+#pragma unroll
+          for (int z = WP - 1; z >= 0; --z)
+#pragma unroll
+            for (int y = VP - 1; y >= 0; --y) {
+              o[2 * d2] = product<half>(even[y], wp[z], o[2 * d2]);
+              o[2 * d2 + 1] = product<half>(odd[y], wp[z], o[2 * d2 + 1]);
+            }
+          if constexpr (VP == 2) __builtin_amdgcn_sched_barrier(0);  // (or the parts of many features are held at once)
         }
+        if constexpr (more) x.load_v(p, rows, waves[wave]);
+      };
+      if constexpr (kHalf) {
+        float least = fmaf(low, c, -shift);  // the least weight's exponent
+        if (__builtin_expect(!__any(least < -16.0f), 1)) sums(std::true_type{});
+        // (Its own branch, its condition out of the compiler's sight: of an if and its else it
+        // keeps two sets of sums.)
+        asm volatile("" : "+v"(least));
+        if (__builtin_expect(__any(least < -16.0f), 0)) sums(std::false_type{});
+      } else {
+        sums(std::false_type{});
       }
-      if constexpr (more) x.load_v(p, rows, waves[wave]);
       __builtin_amdgcn_sched_barrier(0);
     };
     if (!WHOLE) __syncthreads();  // (the sweep before's results are read)
@@ -761,13 +812,13 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
       const float a = __builtin_amdgcn_exp2f(Ms[w][orow] - shift);
       sum += a * Ls[w][orow];
 #pragma unroll
-      for (int e = 0; e < E / 4; ++e) acc[e] += a * *reinterpret_cast<const f32x4*>(&Os[w][orow][col + 4 * e]);
+      for (int e = 0; e < E / 4; ++e) acc[e] += a / kTimes * *reinterpret_cast<const f32x4*>(&Os[w][orow][col + 4 * e]);
     }
     if (slot >= 0) {
       const int64_t to = (int64_t)slot * kRows + orow;
 #pragma unroll
       for (int e = 0; e < E / 4; ++e) *reinterpret_cast<f32x4*>(p.part + to * D + col + 4 * e) = acc[e];
-      if (col == 0) reinterpret_cast<f32x2*>(p.part_ml)[to] = f32x2{mx - kBias, sum};
+      if (col == 0) reinterpret_cast<f32x2*>(p.part_ml)[to] = f32x2{mx, sum};
       continue;
     }
     const int jo = thd::quotient(all, p.by_group), ho = hk * p.group + all - jo * p.group;
@@ -778,7 +829,7 @@ __global__ __launch_bounds__(WHOLE ? 512 : 256, waves_of(D, SINGLE, WHOLE)) void
       if (EXACT || col + 4 * e < p.head_dim)
         *reinterpret_cast<u32x2_any*>(out + 4 * e) =
             u32x2{rounded2<F16>(acc[e][0] * inv, acc[e][1] * inv), rounded2<F16>(acc[e][2] * inv, acc[e][3] * inv)};
-    if (col == 0 && p.lse) p.lse[((int64_t)b * p.seq + jo) * p.heads + ho] = (mx - kBias + log2f(sum)) * kLn2;
+    if (col == 0 && p.lse) p.lse[((int64_t)b * p.seq + jo) * p.heads + ho] = (mx + log2f(sum)) * kLn2;
     if (WHOLE) return;
   }
 }
@@ -900,7 +951,7 @@ int launch(const th_paged_desc* d, th_launch** out) {
   const int64_t keys = (int64_t)d->table_pages * cache.page, sweeps = (int64_t)a.sweeps * d->batch;
   // As many workgroups as run at once (where that cuts the line in eight or more; otherwise four
   // times as many, so that the last round counts for little), or as there are steps if that is fewer.
-  const int64_t resident = (int64_t)th::ctx().prop.multiProcessorCount * waves_of(D, SINGLE, WHOLE);
+  const int64_t resident = (int64_t)th::ctx().prop.multiProcessorCount * waves_of(D, CT, SINGLE, WHOLE);
   int64_t shares = resident / a.sweeps;
   if (shares < 8) shares = (4 * resident + a.sweeps - 1) / a.sweeps;
   if (shares >= 64) shares -= shares % 8;

@@ -486,3 +486,69 @@ def test_decoding_as_it_is_used(target, dtype, e4m3, page):
     graph = target.capture(launches)
     for _ in range(steps):
         step(arrays, lambda: target.replay(graph), 1)
+
+
+@pytest.mark.parametrize("dtype,e4m3", [("f16", False), ("bf16", False), ("f16", True), ("bf16", True)])
+@pytest.mark.parametrize("S,page,cap", [(1, 16, 200), (2, 7, 300), (1, 16, 2500), (3, 7, 2500)])
+def test_small_weights_beside_a_large_one(target, dtype, e4m3, S, page, cap):
+    """One key of score 32 whose value is 0, the others between -4 and 6 with values up to thousands: the
+    output is the small weights' alone, 2^-37 to 2^-52 of the large one.  Each is within `score` +
+    2^-21 of itself as everywhere (the scores' own products are exact), so the weighted mean within twice that
+    of the weighted sizes of the values, 0 for the large one's."""
+    announce("paged small weights", dtype, e4m3, S, page, cap)
+    B, H, KV, D = 2, 4, 2, 64
+    c = Paged(B, cap, KV, D, page, dtype, e4m3)
+    gen = torch.Generator(device="cuda").manual_seed(cap + S)
+    k, v = torch.zeros(c.pages, page, KV, D, device="cuda"), rows(gen, dtype, c.pages, page, KV, D, spread=False).float().abs() * 2.0 ** 12
+    k[..., 0] = torch.rand(k.shape[:-1], device="cuda", generator=gen) * 10 - 4
+    for b in range(B):
+        k[c.where(b, 5)][:, 0], v[c.where(b, 5)] = 32.0, 0.0
+    for name, x in (("k", k), ("v", v)):
+        x = x.to(TYPES[dtype])
+        if e4m3:
+            codes, scales = interpret.e4m3_rows(_np(x), dtype == "f16")
+            getattr(c, name).copy_(torch.from_numpy(codes))
+            getattr(c, name + "s").copy_(torch.from_numpy(scales))
+        else:
+            getattr(c, name).copy_(x)
+    q = torch.zeros(B, S, H, D, device="cuda", dtype=TYPES[dtype])
+    q[..., 0] = 1.0
+    o, lse = torch.empty_like(q), torch.empty(B, S, H, device="cuda")
+    n = [cap, cap - 31]
+    _attend(c, q, o, lse, ints(*n), scale=1.0)()
+    torch.cuda.synchronize()
+    k, v = c.sequences(cap), c.sequences(cap, "v")
+    want, _, _ = interpret.paged_attention(_np(q), k, v, n, scale=1.0)
+    size, _, _ = interpret.paged_attention(_np(q), k, np.abs(v), n, scale=1.0)
+    score = 32.0 * ((D + 8) * 2.0 ** -24 + 2.0 ** -22)
+    limit = 2 * (score + 2.0 ** -21 + (cap / 128 + 40) * 2.0 ** -24) * size + HALF_STEP[dtype] * np.abs(want)
+    limit += 2.0 ** -25 if dtype == "f16" else 0.0  # (half a step below fp16's normals)
+    off = np.abs(_np(o) - want)
+    assert (want[..., 1:] > 0).all() and (off <= limit).all(), (off / limit).max()
+    if not e4m3:  # infinite values under small weights: infinite outputs, the others' bits as they were
+        o2, lse2 = torch.empty_like(o), torch.empty_like(lse)
+        c.v[c.where(0, 7)][0, 9], c.v[c.where(1, cap - 60)][1, 40] = float("inf"), -float("inf")
+        _attend(c, q, o2, lse2, ints(*n), scale=1.0)()
+        torch.cuda.synchronize()
+        assert torch.isposinf(o2[0, :, :2, 9]).all() and torch.isneginf(o2[1, :, 2:, 40]).all()
+        o2[0, :, :2, 9], o2[1, :, 2:, 40] = o[0, :, :2, 9], o[1, :, 2:, 40]
+        assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("page", [1, 16])
+def test_every_fp16_value_comes_out_itself(target, page):
+    """One key, so its weight is 1: every finite value, both infinities and every NaN."""
+    announce("paged fp16 values", page)
+    codes = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(256, 1, 1, 256).view(torch.float16)
+    c = Paged(256, 1, 1, 256, page, "f16")
+    c.k.zero_()
+    for b in range(256):
+        c.v[c.where(b, 0)] = codes[b, 0].cuda()
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q = rows(gen, "f16", 256, 1, 1, 256, spread=False)
+    o, n = torch.empty_like(q), ints(*[1] * 256)
+    _attend(c, q, o, None, n)()
+    torch.cuda.synchronize()
+    o, want = o.cpu(), codes.view(256, 1, 1, 256)
+    assert torch.equal(o.isnan(), want.isnan())
+    assert torch.equal(o[~want.isnan()], want[~want.isnan()])
