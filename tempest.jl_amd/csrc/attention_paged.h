@@ -992,6 +992,7 @@ int launch(const th_paged_desc* d, th_launch** out) {
                            pages + TH_OFFSET(th::Pages, counts)};
   for (int v = 0; v < 10; ++v)
     for (int kk = k; kk <= end; ++kk) b.ref(v, kk, offs[v]);
+  b.element(0, 2), b.element(1, 2);
   b.align(3, 16), b.align(4, 16);
   // All the cache there is room for: how much is held only the device knows.
   const double bytes = CT == kE4m3 ? 33.0 / 32 : 2, D0 = cache.head_dim, all = (double)d->batch * d->seq * d->heads;

@@ -213,6 +213,7 @@ int build(const th_cache_desc* d, bool write, th_launch** out) {
                           TH_OFFSET(CacheArgs, pages) + TH_OFFSET(th::Pages, lengths),
                           TH_OFFSET(CacheArgs, pages) + TH_OFFSET(th::Pages, counts)};
   for (int v = 0; v < values; ++v) b.ref(v, k, offs[v]);
+  b.element(0, 2), b.element(1, 2);
   b.align(2, 16), b.align(3, 16);
   // Every row there is room for: how many there are only the device knows.
   const double rows = (double)d->batch * d->seq * c.heads;

@@ -294,6 +294,7 @@ int build(const th_rotary_desc* d, th_launch** out) {
                           TH_OFFSET(RotaryArgs, positions),
                           TH_OFFSET(RotaryArgs, freqs)};
   for (int i = 0; i < 6; ++i) b.ref(i, k, offs[i]);
+  for (int i = 0; i < 4; ++i) b.element(i, size);
   const double n = (double)a.tokens * (d->heads + d->kv_heads);
   b.work(2.0 * size * n * d->head_dim + 4.0 * a.tokens * d->axes, 6.0 * n * half, blocks);
   *out = b.release();

@@ -147,6 +147,8 @@ class Builder {
   void ref(int v, int k, size_t offset) { l_->values[v].push_back(Ref{k, (uint32_t)offset}); }
   // Value `v` must stay aligned to `bytes` when it is repointed.
   void align(int v, uint32_t bytes) { l_->align[v] = std::max(l_->align[v], bytes); }
+  // Value `v` may lie at any of its elements, of `bytes` each (without this: 4).
+  void element(int v, uint32_t bytes) { l_->align[v] = bytes; }
   void own(void* p) { l_->owned.push_back(p); }
   // Reserve `bytes` of the launch's workspace (256-byte aligned pieces, laid
   // out in order); returns the piece's offset in it.

@@ -552,3 +552,27 @@ def test_every_fp16_value_comes_out_itself(target, page):
     o, want = o.cpu(), codes.view(256, 1, 1, 256)
     assert torch.equal(o.isnan(), want.isnan())
     assert torch.equal(o[~want.isnan()], want[~want.isnan()])
+
+
+@pytest.mark.parametrize("cap", [200, 3000])
+def test_repointed_to_odd_elements(target, cap):
+    """q and o at an odd element, given after the launch was built; the cache's arrays stay at 16 bytes."""
+    from tempest_hip import HIPError
+    announce("paged odd elements", cap)
+    B, S, H, KV, D = 2, 2, 4, 2, 64
+    c = Paged(B, cap, KV, D, 16, "bf16")
+    gen = torch.Generator(device="cuda").manual_seed(cap)
+    _fill(c, gen, cap)
+    q, o, lse = rows(gen, "bf16", B, S, H, D, spread=False), torch.zeros(B, S, H, D, device="cuda", dtype=torch.bfloat16), torch.zeros(B, S, H, device="cuda")
+    n = ints(cap, cap // 3)
+    f = _attend(c, q, o, lse, n)
+    q2 = rows(gen, "bf16", B, S, H, D, spread=False, offset=3)
+    o2 = torch.zeros(B * S * H * D + 1, device="cuda", dtype=torch.bfloat16)[1:].view(B, S, H, D)
+    f.repoint("q", q2.data_ptr())
+    f.repoint("o", o2.data_ptr())
+    f()
+    torch.cuda.synchronize()
+    _check(c, q2, o2, lse, n)
+    for name, at in (("q", q2.data_ptr() + 1), ("table", c.table.data_ptr() + 2), ("v_cache", c.v.data_ptr() + 8)):
+        with pytest.raises(HIPError):
+            f.repoint(name, at)

@@ -232,3 +232,36 @@ def test_a_cache_past_32_bits(target):
     codes, scales = interpret.e4m3_rows(x.double().cpu().numpy())
     assert torch.equal(out.double().cpu(), torch.from_numpy(interpret.e4m3_held(codes, scales)))
     assert torch.equal(k[33999].cpu(), torch.from_numpy(codes[0, :64]))
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_repointed_to_odd_elements(target, e4m3):
+    """Dense rows at an odd element, given after the launch was built; the cache's arrays stay at 16 bytes."""
+    import tempest_hip.launch as L
+    from tempest_hip import HIPError
+    announce("cache odd elements", e4m3)
+    B, S, KV, D, page = 2, 11, 2, 64, 4
+    c = Paged(B, S, KV, D, page, "bf16", e4m3)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    k, v = rows(gen, "bf16", B, S, KV, D), rows(gen, "bf16", B, S, KV, D)
+    n = ints(S, S)
+    write = L.cache_write(c.cache, B, S, k.data_ptr(), v.data_ptr(), c.table.data_ptr(), n.data_ptr(), c.width)
+    read = L.cache_read(c.cache, B, S, k.data_ptr(), v.data_ptr(), c.table.data_ptr(), n.data_ptr(), c.width)
+    k2, v2 = rows(gen, "bf16", B, S, KV, D, offset=1), rows(gen, "bf16", B, S, KV, D, offset=3)
+    out = [torch.zeros(B * S * KV * D + 1, device="cuda", dtype=torch.bfloat16)[1:].view(B, S, KV, D) for _ in range(2)]
+    write.repoint("k", k2.data_ptr())
+    write.repoint("v", v2.data_ptr())
+    read.repoint("k", out[0].data_ptr())
+    read.repoint("v", out[1].data_ptr())
+    write()
+    read()
+    torch.cuda.synchronize()
+    for x, t in zip((k2, v2), out):
+        want = x.double().cpu().numpy()
+        if e4m3:
+            want = interpret.e4m3_held(*interpret.e4m3_rows(want))
+        assert torch.equal(t.double().cpu(), torch.from_numpy(want))
+    with pytest.raises(HIPError):
+        write.repoint("k", k2.data_ptr() + 1)
+    with pytest.raises(HIPError):
+        write.repoint("k_cache", c.k.data_ptr() + 8)

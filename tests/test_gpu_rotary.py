@@ -113,6 +113,31 @@ def test_rotary_strides_and_broadcast_positions(target):
     assert (yq[..., D:] == 3.0).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rotary_repointed_to_odd_elements(target, dtype):
+    import tempest_hip.launch as L
+    from tempest_hip import HIPError
+    announce("rotary odd elements", dtype)
+    B, S, H, KV, D = 2, 9, 4, 2, 64
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    dt = TYPES[dtype]
+    q, k, yq, yk = (_array(gen, dt, B, S, n, D) for n in (H, KV, H, KV))
+    positions = torch.randint(0, 9000, (B, S, 1), dtype=torch.int32, device="cuda", generator=gen)
+    freqs = _freqs(32)
+    f = L.rotary(B, S, H, KV, D, q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), positions.data_ptr(),
+                 freqs.data_ptr(), dtype=_dtype(dtype))
+    odd = {n: _array(gen, dt, B, S, h, D, offset=at) for n, h, at in (("q", H, 1), ("k", KV, 3), ("q_out", H, 5), ("k_out", KV, 1))}
+    for n, t in odd.items():
+        f.repoint(n, t.data_ptr())
+    f()
+    torch.cuda.synchronize()
+    _check(odd["q_out"], odd["q"], positions, freqs, [32], False, False, dtype)
+    _check(odd["k_out"], odd["k"], positions, freqs, [32], False, False, dtype)
+    for n in ("q", "positions", "freqs"):  # between elements there is none
+        with pytest.raises(HIPError):
+            f.repoint(n, q.data_ptr() + (1 if n == "q" else 2))
+
+
 def test_rotary_far_positions(target):
     """Positions across all of int32 keep their turn: at 2^31 of the first
     pair 3.4e8 turns, fp64 leaves 2^-24 of one (the oracle's own angle, in radians, as much)."""
