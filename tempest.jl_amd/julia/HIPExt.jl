@@ -922,8 +922,10 @@ end
 # No program of Tempest's spells these as one group (a rotary turn is a pointwise
 # group of its own, a page a gathered read, a cache's write a fold by key that
 # writes), so no template claims them: a host that serves a model builds their launches
-# and runs them beside a compiled program's, or records them with it.  Arrays are
-# (features, heads, positions, batch) device arrays whose features are adjacent.
+# and runs them between a compiled program's calls.  Arrays are (features, heads,
+# positions, batch) device arrays whose features are adjacent.  A launch's values keep the
+# header's numbers: `repoint!(launch, i, array)` moves value `i` to an array laid out as the one it was
+# built on, which the caller keeps.
 
 struct RotaryDesc
     dtype::Int32; batch::Int32; seq::Int32; heads::Int32; kv_heads::Int32; head_dim::Int32; rotary_dim::Int32
@@ -961,6 +963,22 @@ paged_dtype(T::Type) = T === Tempest.BFloat16 ? Int32(1) : throw(ArgumentError("
 buffer_address(x) = x === nothing ? C_NULL : Ptr{Cvoid}(device_address(x))
 # An array's strides along its axes 2, 3 and 4.
 row_strides(x) = (Int64(stride(x, 2)), Int64(stride(x, 3)), Int64(stride(x, 4)))
+# The operands of a launch of `n` values that are numbered as the header numbers them.
+by_value(n) = Tuple{Int, Int, Int, DataType}[(i, i, 0, UInt8) for i in 0:(n - 1)]
+
+# What the library cannot see behind an address: element types, sizes, what lies side by side.
+held(ok, what) = ok || throw(ArgumentError(what))
+adjacent(x) = size(x, 1) == 1 || stride(x, 1) == 1
+dense(x) = all(i -> size(x, i) == 1 || stride(x, i) == prod(size(x)[1:(i - 1)]), 1:ndims(x))
+alike(x, y) = eltype(x) === eltype(y) && size(x) == size(y) && all(i -> size(x, i) == 1 || stride(x, i) == stride(y, i), 1:4)
+scales_fit(s, k) = eltype(s) === UInt8 && adjacent(s) && 32 * size(s, 1) == size(k, 1) &&
+    all(i -> size(s, i) == size(k, i) && (size(k, i) == 1 || 32 * stride(s, i) == stride(k, i)), 2:4)
+integers(x, n) = eltype(x) === Int32 && dense(x) && length(x) == n
+function check_pages(table, lengths, counts, batch)
+    held(integers(table, size(table, 1) * batch) && size(table, 2) == batch, "table must be a dense Int32 array, (pages of a sequence, batch)")
+    held(integers(lengths, batch), "lengths must be Int32, one for each sequence")
+    held(counts === nothing || integers(counts, batch), "counts must be Int32, one for each sequence")
+end
 
 """
     rotary(t, q, k, q_out, k_out, positions, freqs; sections, pairs = false, inverse = false)
@@ -973,6 +991,11 @@ gradient.
 function rotary(t::HIPTarget, q, k, q_out, k_out, positions, freqs; sections = (length(freqs),), pairs = false,
                 inverse = false)
     kk, ko = k === nothing ? (q, q_out) : (k, k_out)
+    held(adjacent(q) && adjacent(q_out) && eltype(q_out) === eltype(q) && size(q_out) == size(q), "q_out must be of q's type and size, features adjacent in both")
+    held(adjacent(kk) && adjacent(ko) && eltype(ko) === eltype(kk) && size(ko) == size(kk), "k_out must be of k's type and size, features adjacent in both")
+    held(eltype(kk) === eltype(q) && size(kk, 1) == size(q, 1) && size(kk, 3) == size(q, 3) && size(kk, 4) == size(q, 4), "k must be of q's type and of its size but for the heads")
+    held(eltype(positions) === Int32 && size(positions, 1) == length(sections) && size(positions, 2) == size(q, 3) && size(positions, 3) == size(q, 4), "positions must be Int32, (axes, positions, batch)")
+    held(eltype(freqs) === Float32 && dense(freqs), "freqs must be a dense Float32 array")
     d = Ref(RotaryDesc(paged_dtype(eltype(q)), size(q, 4), size(q, 3), size(q, 2), k === nothing ? 0 : size(k, 2),
         size(q, 1), 2length(freqs), length(sections), ntuple(i -> Int32(get(sections, i, 0)), 4),
         (pairs ? 1 : 0) | (inverse ? 2 : 0), 0, buffer_address(q), buffer_address(k), buffer_address(q_out), buffer_address(k_out),
@@ -980,7 +1003,7 @@ function rotary(t::HIPTarget, q, k, q_out, k_out, positions, freqs; sections = (
         (Int64(stride(positions, 1)), Int64(stride(positions, 2)), Int64(stride(positions, 3)))))
     out = Ref{Ptr{Cvoid}}()
     check(ccall((:th_build_rotary, LIB), Cint, (Ptr{RotaryDesc}, Ptr{Ptr{Cvoid}}), d, out), "th_build_rotary")
-    HIPLaunch(out[], Any[q, k, q_out, k_out, positions, freqs], Tuple{Int, Int, Int, DataType}[], t.pool)
+    HIPLaunch(out[], Any[q, k, q_out, k_out, positions, freqs], by_value(6), t.pool)
 end
 
 """
@@ -994,16 +1017,27 @@ struct PagedCache
     v::Any
     k_scales::Any
     v_scales::Any
-    PagedCache(k, v; k_scales = nothing, v_scales = nothing) = new(k, v, k_scales, v_scales)
+    function PagedCache(k, v; k_scales = nothing, v_scales = nothing)
+        held(adjacent(k), "a cache's features must be adjacent")
+        held(alike(v, k), "a cache's v must be of its k's type, size and strides")
+        held(eltype(k) !== UInt8 || k_scales !== nothing && v_scales !== nothing, "e4m3 codes need k_scales and v_scales")
+        held(eltype(k) !== UInt8 || scales_fit(k_scales, k) && scales_fit(v_scales, v), "scales must be UInt8, a byte for each 32 features, their strides the codes' / 32")
+        new(k, v, k_scales, v_scales)
+    end
 end
 paged_dtype(c::PagedCache) = eltype(c.k) === UInt8 ? Int32(5) : paged_dtype(eltype(c.k))
 ccache(c::PagedCache) = CCache(paged_dtype(c), size(c.k, 2), size(c.k, 1), size(c.k, 3), size(c.k, 4), 0,
     buffer_address(c.k), buffer_address(c.v), buffer_address(c.k_scales), buffer_address(c.v_scales), row_strides(c.k))
 paged_values(c::PagedCache) = Any[c.k, c.v, c.k_scales, c.v_scales]
 
-cache_desc(c::PagedCache, k, v, table, lengths, counts) = Ref(CacheDesc(ccache(c), paged_dtype(eltype(k)), size(k, 4),
-    size(k, 3), size(table, 1), buffer_address(k), buffer_address(v), row_strides(k), buffer_address(table), buffer_address(lengths),
-    buffer_address(counts)))
+function cache_desc(c::PagedCache, k, v, table, lengths, counts)
+    held(adjacent(k) && size(k, 1) == size(c.k, 1) && size(k, 2) == size(c.k, 2), "k must hold the cache's heads, features adjacent")
+    held(alike(v, k), "v must be of k's type, size and strides")
+    check_pages(table, lengths, counts, size(k, 4))
+    Ref(CacheDesc(ccache(c), paged_dtype(eltype(k)), size(k, 4),
+        size(k, 3), size(table, 1), buffer_address(k), buffer_address(v), row_strides(k), buffer_address(table), buffer_address(lengths),
+        buffer_address(counts)))
+end
 
 """
     cache_write(t, cache, k, v, table, lengths; counts = nothing)
@@ -1015,12 +1049,12 @@ sequences back: `table` (Int32, (pages of a sequence, batch)), `lengths` and `co
 function cache_write(t::HIPTarget, cache::PagedCache, k, v, table, lengths; counts = nothing)
     d, out = cache_desc(cache, k, v, table, lengths, counts), Ref{Ptr{Cvoid}}()
     check(ccall((:th_build_cache_write, LIB), Cint, (Ptr{CacheDesc}, Ptr{Ptr{Cvoid}}), d, out), "th_build_cache_write")
-    HIPLaunch(out[], [paged_values(cache); Any[k, v, table, lengths, counts]], Tuple{Int, Int, Int, DataType}[], t.pool)
+    HIPLaunch(out[], [paged_values(cache); Any[k, v, table, lengths, counts]], by_value(9), t.pool)
 end
 function cache_read(t::HIPTarget, cache::PagedCache, k, v, table, lengths)
     d, out = cache_desc(cache, k, v, table, lengths, nothing), Ref{Ptr{Cvoid}}()
     check(ccall((:th_build_cache_read, LIB), Cint, (Ptr{CacheDesc}, Ptr{Ptr{Cvoid}}), d, out), "th_build_cache_read")
-    HIPLaunch(out[], [paged_values(cache); Any[k, v, table, lengths]], Tuple{Int, Int, Int, DataType}[], t.pool)
+    HIPLaunch(out[], [paged_values(cache); Any[k, v, table, lengths]], by_value(8), t.pool)
 end
 
 """
@@ -1030,15 +1064,17 @@ The launch of attention of the sequences' last positions `q` over the cache, int
 """
 function paged_attention(t::HIPTarget, cache::PagedCache, q, o, table, lengths; lse = nothing, counts = nothing,
                          causal = true, window = 0, scale = 0)
-    row_strides(o) == row_strides(q) || throw(ArgumentError("o must be laid out as q"))
+    held(adjacent(q) && size(q, 1) == size(cache.k, 1), "q must hold heads of the cache's size, features adjacent")
+    held(alike(o, q), "o must be of q's type, size and strides")
+    held(lse === nothing || eltype(lse) === Float32 && dense(lse) && length(lse) == size(q, 2) * size(q, 3) * size(q, 4), "lse must be a dense Float32 array, (heads, positions, batch)")
+    check_pages(table, lengths, counts, size(q, 4))
     d = Ref(PagedDesc(ccache(cache), paged_dtype(eltype(q)), size(q, 4), size(q, 2), size(q, 3), size(table, 1),
         causal, window, scale, buffer_address(q), buffer_address(o), buffer_address(lse), row_strides(q), buffer_address(table), buffer_address(lengths),
         buffer_address(counts)))
     out = Ref{Ptr{Cvoid}}()
     check(ccall((:th_build_attention_paged, LIB), Cint, (Ptr{PagedDesc}, Ptr{Ptr{Cvoid}}), d, out),
           "th_build_attention_paged")
-    HIPLaunch(out[], [paged_values(cache); Any[q, o, lse, table, lengths, counts]], Tuple{Int, Int, Int, DataType}[],
-        t.pool)
+    HIPLaunch(out[], [paged_values(cache); Any[q, o, lse, table, lengths, counts]], by_value(10), t.pool)
 end
 
 # ---- the floor: any group, generated -----------------------------------------------------
