@@ -912,17 +912,21 @@ __global__ __launch_bounds__(1024) void paged_attn_join(PagedArgs p) {
 // round of workgroups waits.  Both measured, whole and in pieces, 32/8 heads of 128 in bf16: one
 // sequence and a table of 500 positions 8.8 and 9.0 us, of 1000 12.7 and 10.0; 24 sequences (192 sweeps, a CU
 // each) of 850 13.7 and 18.1, of 1400 21.5 and 22.6; 64 sequences of 750 28.6 and 30.7, of
-// 1000 38.7 and 34.9.  The row's bytes weigh as the borders of 64, 128 and 256 features say (few
-// sweeps 1000, 650 and 370 positions in bf16, 800 of 128 in e4m3; a CU each 2300, 1500 and 850, 1800).
-// Few sweeps in pages not in sixteens, whose pieces take longer to start: one sequence of 750, pages of
-// five, 10.6 whole and 10.7; proposals of 12/4 heads of 64 in a window of 1000, pages of seven, 11.3 and 13.2.
-inline bool whole_sweeps(const th_paged_desc* d) {
+// 1000 38.7 and 34.9.  A position weighs 96 and 2 for each of the kernel's D features (e4m3 1.5), which
+// brings the borders of 64, 128 and 256 features, and of head dims between, together.
+// Few sweeps, 52 shapes (those features, bf16, fp16 and e4m3, pages of 5, 7, 16 and 24, one to twelve
+// sequences, tables and windows of 500 to 1800 positions): whole takes 0.88 of the time of pieces at a
+// weight of 190000, 0.95 at 230000, 1.06 at 270000, 1.11 at 310000.  Pages in sixteens or not make no difference;
+// windows, whose sweeps are all as long, cross at 270000, tables filled to all degrees at 235000.
+// A CU each (10 shapes), whole takes 0.87 at 460000, 1.01 at 560000; more sweeps (10), 0.88 at 230000, 1.01 at 290000.
+template <int D>
+bool whole_sweeps(const th_paged_desc* d) {
   int64_t keys = (int64_t)d->table_pages * d->cache.page;
   if (d->window > 0) keys = std::min<int64_t>(keys, (int64_t)d->window + d->seq + 2 * kBlock);
   const int64_t sweeps = ((int64_t)d->seq * (d->heads / d->cache.heads) + kRows - 1) / kRows * d->cache.heads * d->batch;
-  const int64_t row = 96 + d->cache.head_dim * (d->cache.dtype == TH_E4M3 ? 3 : 4) / 2;
+  const int64_t row = 96 + D * (d->cache.dtype == TH_E4M3 ? 3 : 4) / 2;
   const int64_t cus = th::ctx().prop.multiProcessorCount;
-  return keys * row <= (8 * sweeps < 3 * cus ? (d->cache.page % 16 ? 1 << 18 : 7 << 15) : sweeps <= cus ? 1 << 19 : 9 << 15);
+  return keys * row <= (8 * sweeps < 3 * cus ? 15 << 14 : sweeps <= cus ? 1 << 19 : 9 << 15);
 }
 
 template <int D, int CT, bool F16, bool EXACT, bool UNIFORM, bool SINGLE, bool WHOLE, bool EARLY>
@@ -1013,7 +1017,7 @@ int launch(const th_paged_desc* d, th_launch** out) {
   // Whole sweeps of several positions of 256 features lack registers, the more with the
   // scalar addresses (12.5 us and 9.3 without, 2 x 64 positions of 8 heads in bf16).
   constexpr bool scalar = UNIFORM && (SINGLE || D < 256);
-  if (!whole_sweeps(d)) return launch<D, EXACT, UNIFORM, SINGLE, false, false>(d, out);
+  if (!whole_sweeps<D>(d)) return launch<D, EXACT, UNIFORM, SINGLE, false, false>(d, out);
   if constexpr (!scalar)
     if (d->window == 0 && d->table_pages <= kEntries) return launch<D, EXACT, scalar, SINGLE, true, true>(d, out);
   return launch<D, EXACT, scalar, SINGLE, true, false>(d, out);

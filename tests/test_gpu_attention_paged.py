@@ -576,3 +576,16 @@ def test_repointed_to_odd_elements(target, cap):
     for name, at in (("q", q2.data_ptr() + 1), ("table", c.table.data_ptr() + 2), ("v_cache", c.v.data_ptr() + 8)):
         with pytest.raises(HIPError):
             f.repoint(name, at)
+
+
+@pytest.mark.parametrize("cap", [640, 720, 800])
+def test_the_split_goes_by_positions_and_features(target, cap):
+    """Whether a sweep is one workgroup's is the same for pages in sixteens and others, and for all head
+    dims that one kernel takes."""
+    announce("paged split", cap)
+    ways = set()
+    for page, D in ((16, 128), (8, 128), (5, 128), (16, 80), (10, 96)):
+        c = Paged(1, cap, 8, D, page, "bf16")
+        q = torch.zeros(1, 1, 32, D, device="cuda", dtype=torch.bfloat16)
+        ways.add("whole" in _attend(c, q, torch.zeros_like(q), None, ints(cap)).describe())
+    assert len(ways) == 1
