@@ -589,3 +589,74 @@ def test_the_split_goes_by_positions_and_features(target, cap):
         q = torch.zeros(1, 1, 32, D, device="cuda", dtype=torch.bfloat16)
         ways.add("whole" in _attend(c, q, torch.zeros_like(q), None, ints(cap)).describe())
     assert len(ways) == 1
+
+
+@pytest.mark.parametrize("B,H,KV,D,page,cap,dtype,e4m3,window", [
+    (100, 2, 1, 8, 1, 2300, "bf16", False, 0), (100, 2, 1, 64, 1, 2400, "f16", False, 2200), (100, 4, 1, 32, 1, 2700, "bf16", True, 0)])
+def test_whole_sweeps_of_more_entries_than_lds_holds(target, B, H, KV, D, page, cap, dtype, e4m3, window):
+    """2048 entries of the table are in LDS at a time: sweeps that take them in two parts, from wherever they start."""
+    lengths = [(211 * i) % (cap + 1) if i % 3 else cap - i for i in range(B)]
+    c = Paged(1, 1, KV, D, 1, dtype, e4m3)
+    q = torch.zeros(B, 1, H, D, device="cuda", dtype=TYPES[dtype])
+    import tempest_hip.launch as L
+    assert "whole" in L.attention_paged(c.cache, B, H, 1, q.data_ptr(), q.data_ptr(), c.table.data_ptr(), c.table.data_ptr(), cap,
+                                        window=window, dtype=c.type).describe()
+    test_paged(target, B, 1, H, KV, D, page, cap, dtype, e4m3, False, lengths, None, {"window": window} if window else {})
+
+
+@pytest.mark.parametrize("B,S,KV,D,page,cap,dtype,e4m3,window", [
+    (3, 1, 1100, 8, 1, 3600, "bf16", False, 0), (3, 1, 1100, 8, 1, 3600, "f16", False, 3100), (4, 1, 1100, 8, 2, 5000, "bf16", False, 0),
+    (3, 2, 1100, 8, 1, 3600, "bf16", False, 0), (3, 1, 1100, 32, 1, 3600, "bf16", True, 0), (2, 1, 2100, 64, 1, 2600, "bf16", False, 0)])
+def test_pieces_of_more_entries_than_lds_holds(target, B, S, KV, D, page, cap, dtype, e4m3, window):
+    """The same where the keys are cut in a few pieces of thousands of positions."""
+    announce("paged long pieces", B, S, KV, D, page, cap, dtype, e4m3, window)
+    c = Paged(B, cap, KV, D, page, dtype, e4m3)
+    gen = torch.Generator(device="cuda").manual_seed(cap + D)
+    if e4m3:  # any codes but NaN's, scales 2^-8..2^-6
+        for t, s in ((c.k, c.ks), (c.v, c.vs)):
+            t.copy_(torch.randint(0, 127, t.shape, device="cuda", generator=gen) + 128 * torch.randint(0, 2, t.shape, device="cuda", generator=gen))
+            s.copy_(torch.randint(119, 122, s.shape, device="cuda", generator=gen))
+    else:
+        _fill(c, gen, cap)
+    q = rows(gen, dtype, B, S, KV, D, spread=False)
+    lengths = [cap - 500 * (b % 2) - b for b in range(B)]
+    n = ints(*lengths)
+    o, lse = torch.full_like(q, 6.0), torch.full((B, S, KV), 6.0, device="cuda")
+    _attend(c, q, o, lse, n, window=window)()
+    torch.cuda.synchronize()
+
+    def held(t, s, b, heads):
+        x = t[c.table[b].long()].reshape(-1, KV, t.shape[-1])[:lengths[b], heads]
+        if not e4m3:
+            return x.double()
+        s = s[c.table[b].long()].reshape(-1, KV, s.shape[-1])[:lengths[b], heads].double()
+        return (x.view(torch.float8_e4m3fn).double().unflatten(-1, (-1, 32)) * torch.exp2(s - 127)[..., None]).flatten(-2)
+    for b in range(B):
+        for h in range(0, KV, 300):
+            heads = slice(h, min(KV, h + 300))
+            k, v = held(c.k, c.ks, b, heads), held(c.v, c.vs, b, heads)
+            for j in range(S):
+                end = lengths[b] - S + j + 1
+                lo = max(0, end - window) if window else 0
+                qj = q[b, j, heads].double()
+                s = (k[lo:end] * qj).sum(-1) * D ** -0.5
+                w = torch.softmax(s, 0)
+                want = (w[..., None] * v[lo:end]).sum(0)
+                score = (qj.abs() * k.abs().amax(0)).sum(-1) * D ** -0.5 * ((D + 8) * 2.0 ** -24 + 2.0 ** -22)
+                rel = 2 * (score + 2.0 ** -21 + (end / 128 + 40) * 2.0 ** -24)
+                limit = rel[:, None] * v.abs().amax(0) + HALF_STEP[dtype] * want.abs() + 2.0 ** -25
+                assert ((o[b, j, heads].double() - want).abs() <= limit).all(), (b, h, j)
+                exact = torch.logsumexp(s, 0)
+                assert ((lse[b, j, heads].double() - exact).abs() <= score + 2.0 ** -20 + 2.0 ** -22 * exact.abs()).all(), (b, h, j)
+
+
+@pytest.mark.parametrize("B,S,H,KV,D,page,cap,dtype,e4m3,lengths,counts,masks", [
+    (2, 1000, 4, 2, 64, 16, 1500, "bf16", False, [1500, 900], [1000, 777], {}),
+    (1, 2500, 2, 1, 128, 16, 3100, "bf16", True, [3100], [2499], {"window": 700}),
+    (2, 700, 6, 2, 64, 7, 1500, "f16", False, [1499, 20], [700, 33], {}),
+    (2, 300, 4, 1, 256, 24, 700, "bf16", False, [700, 300], None, {"causal": False}),
+    (2, 65535, 1, 1, 8, 16, 400, "bf16", False, [300, 400], [300, 0], {}),
+    (1, 65535, 3, 1, 96, 16, 400, "f16", True, [390], [37], {"window": 50})])
+def test_many_new_positions(target, B, S, H, KV, D, page, cap, dtype, e4m3, lengths, counts, masks):
+    """A prompt's next piece over its context: many tiles of rows a head, ragged counts, the most positions there may be."""
+    test_paged(target, B, S, H, KV, D, page, cap, dtype, e4m3, False, lengths, counts, masks)
