@@ -7,7 +7,7 @@
 // in LDS, then each turns V pairs at a time, 16 bytes of either half.
 //
 // The angle is position * frequency, in turns t = position * (freq / 2 pi) in
-// fp64 (two roundings: off by at most 2^-52 t, so by 2^-21 of a turn at 2^31 turns);
+// fp64 (1 / 2 pi is off by 0.56 * 2^-53 of itself, two roundings: by at most 1.28 * 2^-52 t, 2^-20 of a turn at 2^31);
 // t - rint(4 t) / 4, in [-1/8, 1/8], is exact and goes on in fp32, where
 // Taylor's polynomials of sin and cos on [-pi/4, pi/4] leave out under 2^-28.
 #include <hip/hip_runtime.h>
@@ -37,13 +37,14 @@ struct RotaryArgs {
   int32_t turning, passing;      // items of a head: turned, copied
   int32_t pass_second;           // features from a copied item's first vector to its second (0: it has one)
   int32_t per_block;             // tokens a workgroup
-  th::Divisor by_seq, by_half;
-  th::Divisor by_token[2], by_head[2];  // items of a token, of a head: turned alone, copied too
+  th::Divisor by_seq, by_half, by_token, by_head;  // (items of a token, of a head)
   float sign;
+  // LEFT: items of a head that would be copied; heads of q and k.
+  int32_t left;
+  th::Divisor by_left, by_heads;
 };
 
-// Whether what passes has to be copied: an array's result lies elsewhere.  The
-// kernel asks, for the arrays may be pointed elsewhere after the launch was built.
+// Whether what passes has to be copied: an array's result lies elsewhere.
 __host__ __device__ __forceinline__ bool moves(const RotaryArray& q, const RotaryArray& k) {
   return q.x != q.y || (k.heads && k.x != k.y);
 }
@@ -116,28 +117,29 @@ __device__ __forceinline__ void store(E* to, const Vec<E, V>& x) {
   __builtin_nontemporal_store(__builtin_bit_cast(words, x), reinterpret_cast<words*>(to));
 }
 
-template <int T, int V, bool PAIRS>
+// LEFT: built with all arrays in place, so that what passes is not among the items; the
+// arrays may since have been pointed elsewhere.  (In place the test is all it costs: 8 x 2048 positions of
+// 16/16 heads, 64 of 128 features turned, 25 us; apart, built so, 54.5.)
+template <int T, int V, bool PAIRS, bool LEFT>
 __global__ __launch_bounds__(256) void rotary(RotaryArgs p) {
   typedef typename Element<T>::type E;
   typedef Vec<E, V> W;
   extern __shared__ float2 turns[];  // [token][pair]: sin, cos
   const int first = blockIdx.x * p.per_block, tokens = min(p.per_block, p.tokens - first);
-  const RotaryArray qa = p.a[0], ka = p.a[1];
-  const bool copy = moves(qa, ka);
-  const th::Divisor by_token = p.by_token[copy], by_head = p.by_head[copy];
-  const int per_head = p.turning + (copy ? p.passing : 0);
-  const int per_token = (qa.heads + ka.heads) * per_head, items = tokens * per_token;
+  const int per_head = p.turning + p.passing;
+  const int per_token = (p.a[0].heads + p.a[1].heads) * per_head, items = tokens * per_token;
   // An item's place: its token of the workgroup's, its features of x and y.
   struct Item {
     const E* x;
     E* y;
     int t, item, f0, f1;
   };
+  const RotaryArray qa = p.a[0], ka = p.a[1];
   auto item_of = [&](int i) {
     Item it;
-    it.t = thd::quotient(i, by_token);
+    it.t = thd::quotient(i, p.by_token);
     const int at = i - it.t * per_token;
-    int head = thd::quotient(at, by_head);
+    int head = thd::quotient(at, p.by_head);
     it.item = at - head * per_head;
     const bool second = head >= qa.heads;
     auto of = [&](auto q, auto k) { return second ? k : q; };  // (scalars both, not loads from where the index says)
@@ -193,17 +195,33 @@ __global__ __launch_bounds__(256) void rotary(RotaryArgs p) {
     store(it.y + it.f1, v);
     it = it2, u = u2, v = v2, i = next;
   }
+  if (LEFT && moves(qa, ka)) {
+    const int heads = qa.heads + ka.heads;
+    for (int i = begin; i < tokens * heads * p.left; i += step) {
+      const int row = thd::quotient(i, p.by_left), t = thd::quotient(row, p.by_heads), head = row - t * heads;
+      const int token = first + t, b = thd::quotient(token, p.by_seq), s = token - b * p.seq;
+      const bool second = head >= qa.heads;
+      const RotaryArray& a = second ? ka : qa;
+      const int h = second ? head - qa.heads : head, f = 2 * p.half + (V + p.pass_second) * (i - row * p.left);
+      const E* from = static_cast<const E*>(a.x) + h * a.xh + s * a.xs + b * a.xb + f;
+      E* to = static_cast<E*>(a.y) + h * a.yh + s * a.ys + b * a.yb + f;
+      u = load<V>(from), v = load<V>(from + p.pass_second);
+      store(to, u);
+      store(to + p.pass_second, v);
+    }
+  }
 }
 
 template <int T, int V>
-const void* kernel_of(bool pairs) {
-  return pairs ? (const void*)rotary<T, V, true> : (const void*)rotary<T, V, false>;
+const void* kernel_of(bool pairs, bool left) {
+  return pairs ? (left ? (const void*)rotary<T, V, true, true> : (const void*)rotary<T, V, true, false>)
+               : (left ? (const void*)rotary<T, V, false, true> : (const void*)rotary<T, V, false, false>);
 }
 template <int T>
-const void* kernel_of(int v, bool pairs) {
+const void* kernel_of(int v, bool pairs, bool left) {
   if constexpr (T != TH_F32)
-    if (v == 8) return kernel_of<T, 8>(pairs);
-  return v == 4 ? kernel_of<T, 4>(pairs) : v == 2 ? kernel_of<T, 2>(pairs) : kernel_of<T, 1>(pairs);
+    if (v == 8) return kernel_of<T, 8>(pairs, left);
+  return v == 4 ? kernel_of<T, 4>(pairs, left) : v == 2 ? kernel_of<T, 2>(pairs, left) : kernel_of<T, 1>(pairs, left);
 }
 
 int check_array(const void* x, void* y, const int64_t* xs, const int64_t* ys, const th_rotary_desc* d, int heads,
@@ -265,24 +283,21 @@ int build(const th_rotary_desc* d, th_launch** out) {
   while (half % v || pass % v) v /= 2;
   const bool pairs = d->flags & TH_ROTARY_PAIRS;
   a.turning = half / v, a.pass_second = pass % (2 * v) == 0 ? v : 0;
-  a.passing = pass / (v + a.pass_second);
-  // The workgroups are sized for where the arrays lie now; any share of the items is right.
-  const int all = d->heads + d->kv_heads;
-  const int64_t per_token = (int64_t)all * (a.turning + (moves(a.a[0], a.a[1]) ? a.passing : 0));
+  const int copied = pass / (v + a.pass_second);
+  (moves(a.a[0], a.a[1]) ? a.passing : a.left) = copied;
+  const int64_t per_token = (int64_t)(d->heads + d->kv_heads) * (a.turning + a.passing);
   TH_REQUIRE(per_token <= (1 << 24), "rotary: heads * head_dim is too large");
   // About four items a thread, at most 8 KB of angles.
   a.per_block = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / per_token, 1024 / half));
   const int64_t blocks = (tokens + a.per_block - 1) / a.per_block;
   TH_REQUIRE(blocks <= 0xffffff, "rotary: batch * seq is too large");  // 2^32 threads
   if (int r = th::require_ready()) return r;
-  a.by_seq = th::divisor(a.seq), a.by_half = th::divisor(a.half);
-  for (int copy = 0; copy < 2; ++copy) {
-    const int per_head = a.turning + copy * a.passing;
-    a.by_head[copy] = th::divisor(per_head), a.by_token[copy] = th::divisor(all * per_head);
-  }
-  const void* fn = d->dtype == TH_F32    ? kernel_of<TH_F32>(v, pairs)
-                   : d->dtype == TH_BF16 ? kernel_of<TH_BF16>(v, pairs)
-                                         : kernel_of<TH_F16>(v, pairs);
+  a.by_seq = th::divisor(a.seq), a.by_half = th::divisor(a.half), a.by_token = th::divisor((int)per_token);
+  a.by_head = th::divisor(a.turning + a.passing);
+  a.by_left = th::divisor(std::max(a.left, 1)), a.by_heads = th::divisor(d->heads + d->kv_heads);
+  const void* fn = d->dtype == TH_F32    ? kernel_of<TH_F32>(v, pairs, a.left > 0)
+                   : d->dtype == TH_BF16 ? kernel_of<TH_BF16>(v, pairs, a.left > 0)
+                                         : kernel_of<TH_F16>(v, pairs, a.left > 0);
   // Few tokens: their items to several workgroups each.
   const int64_t slices = blocks >= 512 ? 1 : std::min<int64_t>((a.per_block * per_token + 255) / 256, 512 / blocks);
   th::Builder b("rotary", 6);
