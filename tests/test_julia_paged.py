@@ -157,7 +157,7 @@ def _rotary(**over):
 
 @pytest.mark.parametrize("over", [
     {}, dict(q_out=Array(HALF, 64, 4, 5, 2, strides=(1, 128, 512, 2560))),
-    dict(q=Array(HALF, 64, 4, 5, 2, strides=(1, 64, 512, 2560))), dict(sections=(32,), positions=Array("Int32", 1, 5, 2))], ids=str)
+    dict(q=Array(HALF, 64, 4, 5, 2, strides=(1, 64, 512, 2560))), dict(sections=(32,), positions=Array("Int32", 1, 5, 2))], ids=lambda o: ",".join(o) or "plain")
 def test_rotary_takes(over):
     assert _rotary(**over) is None
 
@@ -184,7 +184,7 @@ OUTER = (1, 1024, 64, 2048)  # heads outside the positions
 @pytest.mark.parametrize("over", [
     {}, dict(k=Array(HALF, 64, 2, 16, 10), v=Array(HALF, 64, 2, 16, 10), k_scales=None, v_scales=None),
     dict(k=Array("UInt8", 64, 2, 16, 10, strides=OUTER), v=Array("UInt8", 64, 2, 16, 10, strides=OUTER),
-         k_scales=Array("UInt8", 2, 2, 16, 10, strides=(1, 32, 2, 64)), v_scales=Array("UInt8", 2, 2, 16, 10, strides=(1, 32, 2, 64)))], ids=str)
+         k_scales=Array("UInt8", 2, 2, 16, 10, strides=(1, 32, 2, 64)), v_scales=Array("UInt8", 2, 2, 16, 10, strides=(1, 32, 2, 64)))], ids=lambda o: ",".join(o) or "plain")
 def test_a_cache_takes(over):
     assert _paged(**over) is None
 
@@ -210,7 +210,7 @@ def _rows(**over):
 
 
 @pytest.mark.parametrize("over", [{}, dict(counts=Array("Int32", 2)), dict(k=Array(HALF, 64, 2, 5, 2, strides=(1, 320, 64, 640)),
-                                                                           v=Array(HALF, 64, 2, 5, 2, strides=(1, 320, 64, 640)))], ids=str)
+                                                                           v=Array(HALF, 64, 2, 5, 2, strides=(1, 320, 64, 640)))], ids=lambda o: ",".join(o) or "plain")
 def test_rows_taken(over):
     assert _rows(**over) is None
 
@@ -229,7 +229,7 @@ def _attention(**over):
 
 
 @pytest.mark.parametrize("over", [{}, dict(lse=Array("Float32", 8, 3, 2), counts=Array("Int32", 2)),
-                                  dict(q=Array(HALF, 64, 8, 1, 2, strides=(1, 64, 9, 512)), o=Array(HALF, 64, 8, 1, 2))], ids=str)
+                                  dict(q=Array(HALF, 64, 8, 1, 2, strides=(1, 64, 9, 512)), o=Array(HALF, 64, 8, 1, 2))], ids=lambda o: ",".join(o) or "plain")
 def test_attention_takes(over):
     assert _attention(**over) is None
 
