@@ -13,7 +13,7 @@
 //     two a workgroup at most, that a second kernel joins by their maxima and sums.
 //     Short tables take no pieces: eight waves a sweep, one launch (whole_sweeps).
 //   - The heads of a piece, whose rows lie side by side, run on one XCD and start a few
-//     workgroups apart: 8 sequences of 8 heads of 128 in e4m3 and 65536 positions 114 us;
+//     workgroups apart: 8 sequences of 8 heads of 128 in e4m3 and 65536 positions 114 us, the join with it;
 //     each head cut by itself 125, the heads side by side in order (all at the same line at
 //     once) 130.
 //   - A wave takes 32 keys at a time.  The next 32's K and V rows are under way in registers
